@@ -151,6 +151,13 @@ def _make_lut(case, g, dev):
     return s
 
 
+def _log_sum(z, temperature):
+    """largest value of each row, logarithm of the sum of exp((z - largest) / temperature)"""
+    top = z.amax(1, keepdim=True)
+    shifted = torch.where(z == -math.inf, z, z - top)
+    return top, torch.log(torch.exp(shifted / temperature).sum(1, keepdim=True))
+
+
 def _make_distill(case, g, dev):
     n, v, k, dt, lay = case["positions"], case["vocab"], case["top"], _DTYPES[case["dtype"]], case["layout"]
     z = (torch.randn((n, v), generator=g, device=dev) * 3.0).to(dt)
@@ -169,12 +176,13 @@ def _make_distill(case, g, dev):
     del z
     if case["dir"] == "fwd":
         s["loss"] = torch.empty(position, device=dev)
-        s["stats"] = torch.empty((n, 2) if lay == "rows" else (2, n), device=dev)
+        s["stats"] = torch.empty((n, 4) if lay == "rows" else (4, n), device=dev)
     else:
         zp, tp, ip = (_by_position(s[a], lay) for a in ("z", "t", "ids"))
-        lse = torch.cat([torch.logsumexp(zp[i:i + 1024].double() / case["temperature"], 1) for i in range(0, n, 1024)])
-        tt = torch.where(ip >= 0, tp.double() / case["temperature"], torch.full(tp.shape, -math.inf, device=dev).double())
-        s["stats"] = _oriented(torch.stack((lse, torch.logsumexp(tt, 1)), 1).float(), lay)
+        tt = torch.where(ip >= 0, tp.double(), torch.full(tp.shape, -math.inf, device=dev).double())
+        parts = [torch.cat(_log_sum(zp[i:i + 1024].double(), case["temperature"]) + _log_sum(tt[i:i + 1024], case["temperature"]), 1)
+                 for i in range(0, n, 1024)]
+        s["stats"] = _oriented(torch.cat(parts).float(), lay)
         # the weight of each position in the cost (the optimizer divides by the batch size)
         s["weight"] = torch.rand(position, generator=g, device=dev) + 0.5
         s["dz"] = torch.empty_like(s["z"])
@@ -244,22 +252,22 @@ def _plain_distill(s, case):
     inv = 1.0 / s["temperature"]
     valid = s["ids"] >= 0
     ids = s["ids"].clamp(min=0).long()
-    z = s["z"].float() * inv
-    t = torch.where(valid, s["t"].float() * inv, torch.full((), -math.inf, device=z.device))
+    some = valid.any(axis, keepdim=True)
+    z = s["z"].float()
+    t = torch.where(valid, s["t"].float(), torch.full((), -math.inf, device=z.device))
     if case["dir"] == "fwd":
         top = z.max(axis, keepdim=True).values
-        lse = top + torch.log(torch.exp(z - top).sum(axis, keepdim=True))
-        some = valid.any(axis, keepdim=True)
-        ttop = torch.where(some, t.max(axis, keepdim=True).values, torch.zeros_like(top))
-        tlse = ttop + torch.log(torch.exp(t - ttop).sum(axis, keepdim=True))
-        logp = torch.where(valid, t - tlse, torch.zeros_like(t))
-        p = torch.where(valid, torch.exp(logp), torch.zeros_like(t))
-        terms = p * (logp - (z.gather(axis, ids) - lse))
-        return (terms * valid).sum(axis, keepdim=True) * s["temperature"] ** 2, torch.cat((lse, tlse), axis)
-    lse, tlse = s["stats"].split(1, axis)
-    some = valid.any(axis, keepdim=True)
-    p = torch.where(valid, torch.exp(t - torch.where(some, tlse, torch.zeros_like(tlse))), torch.zeros_like(t))
-    d = torch.where(some, torch.exp(z - lse), torch.zeros_like(z)).scatter_add_(axis, ids, -p)
+        z = (z - top) * inv
+        log_sum = torch.log(torch.exp(z).sum(axis, keepdim=True))
+        ttop = t.max(axis, keepdim=True).values
+        t = (t - torch.where(some, ttop, torch.zeros_like(ttop))) * inv
+        tlog_sum = torch.log(torch.exp(t).sum(axis, keepdim=True))
+        logp = torch.where(valid, t - tlog_sum, torch.zeros_like(t))
+        terms = torch.where(valid, torch.exp(logp) * (logp - (z.gather(axis, ids) - log_sum)), torch.zeros_like(t))
+        return terms.sum(axis, keepdim=True) * s["temperature"] ** 2, torch.cat((top, log_sum, ttop, tlog_sum), axis)
+    top, log_sum, ttop, tlog_sum = s["stats"].split(1, axis)
+    p = torch.where(valid, torch.exp((t - ttop) * inv - tlog_sum), torch.zeros_like(t))
+    d = torch.where(some, torch.exp((z - top) * inv - log_sum), torch.zeros_like(z)).scatter_add_(axis, ids, -p)
     return (d * (s["weight"] * s["temperature"])).to(s["z"].dtype)
 
 
@@ -317,7 +325,7 @@ def work(case):
         live = n * (0.9 if case["pad"] else 1.0)
         return {"bytes": 4 * n + ((words + n) if fwd else (live + v)) * e * size, "flops": n * e}
     v, k = case["vocab"], case["top"]
-    return {"bytes": (1 if fwd else 2) * n * v * size + n * k * (4 + size) + 12 * n, "flops": 6 * n * v}
+    return {"bytes": (1 if fwd else 2) * n * v * size + n * k * (4 + size) + 20 * n, "flops": 6 * n * v}
 
 
 # ---- the definitions in 64 bits, position by position -------------------------------------
@@ -384,17 +392,18 @@ def _exact_distill(s, case):
         ti = ti.masked_fill(~real, -math.inf)
         if case["dir"] == "fwd":
             log_q = torch.log_softmax(zi, 1)
-            lse, tlse = torch.logsumexp(zi, 1), torch.logsumexp(ti, 1)
+            best, tbest = zi.max(1).values, ti.max(1).values
+            rest, trest = torch.logsumexp(zi, 1) - best, torch.logsumexp(ti, 1) - tbest.clamp(min=-1e300)
             log_p = torch.log_softmax(ti, 1)
             cross = log_p - torch.gather(log_q, 1, ki.clamp(0, v - 1))
             terms = torch.where(real, log_p.exp() * cross, torch.zeros_like(cross))
-            parts.append((tau * tau * terms.sum(1), torch.stack((lse, tlse), 1)))
+            parts.append((tau * tau * terms.sum(1), torch.stack((best * tau, rest, tbest * tau, trest), 1)))
         else:
-            lse, tlse = _by_position(s["stats"], lay)[i:i + 1024].double().unbind(1)
+            best, rest, tbest, trest = _by_position(s["stats"], lay)[i:i + 1024].double().unbind(1)
             some = real.any(1)
             d = torch.zeros_like(zi)
-            d[some] = (zi[some] - lse[some, None]).exp()
-            p = torch.where(real, (ti - tlse[:, None]).exp(), torch.zeros_like(ti))
+            d[some] = (zi[some] - (best / tau + rest)[some, None]).exp()
+            p = torch.where(real, (ti - (tbest / tau + trest)[:, None]).exp(), torch.zeros_like(ti))
             row, col = real.nonzero(as_tuple=True)
             d.index_put_((row, ki[row, col]), -p[row, col], accumulate=True)
             parts.append((d * (_by_position(s["weight"], lay)[i:i + 1024].double() * tau),))

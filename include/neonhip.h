@@ -275,6 +275,75 @@ int nh_lut_bprop(void* dW, const void* error_t, const int32_t* ids, int itemsize
                  uint32_t vocab, size_t ld_dw, size_t ld_err, int32_t pad_idx, void* workspace, size_t workspace_bytes,
                  void* stream);
 
+/* ---- language-model operators -------------------------------------------------
+ * Layer normalisation, embedding lookup and distillation from a teacher's top
+ * logits, forward and backward; the reference has batch normalisation, a lookup
+ * table and cross-entropy only (neon/backends/nervanagpu.py:2463-2660,
+ * neon/transforms/cost.py:112-173).
+ *
+ * `dtype` names the storage of the large tensors; statistics, gamma, beta,
+ * their gradients, losses and weights are fp32.  `axis` is the axis that a
+ * position's values lie along in a row-major matrix: 1 = (positions, features),
+ * 0 = (features, positions).  Leading dimensions are elements between stored
+ * lines; the lines themselves are dense and may start at any element.
+ * Workspaces are device scratch, need not be initialised, and belong to one
+ * call at a time: calls that may overlap (other streams, captured graphs) need
+ * one each.  No call allocates, synchronises or records a memset.  Arguments
+ * are checked before anything is launched.  The kernels run on the device of
+ * nh_init.                                                                     */
+#define NH_T_F32 0
+#define NH_T_F16 1
+#define NH_T_BF16 2
+
+/* y = gamma * (x - mean) / sqrt(var + eps) + beta, mean and var (biased) of each
+ * position over its features, written to mean[positions], var[positions];
+ * gamma, beta hold one value per feature.  y may be x.                         */
+size_t nh_ln_workspace_bytes(int backward, int dtype, int axis, size_t features, size_t positions);
+int nh_ln_fprop(void* y, float* mean, float* var, const void* x, const float* gamma, const float* beta, float eps,
+                int dtype, int axis, size_t features, size_t positions, size_t ld_x, size_t ld_y,
+                void* workspace, size_t workspace_bytes, void* stream);
+/* With h = (x - mean) / sqrt(var + eps), u = gamma * dy:
+ *   dx = (u - mean_f(u) - h mean_f(u h)) / sqrt(var + eps),
+ *   dgamma = sum over positions of dy h, dbeta = sum over positions of dy
+ * (overwritten; added up in a fixed order).  dx may be dy or x.                */
+int nh_ln_bprop(void* dx, float* dgamma, float* dbeta, const void* dy, const void* x, const float* mean, const float* var,
+                const float* gamma, float eps, int dtype, int axis, size_t features, size_t positions, size_t ld_x,
+                size_t ld_dy, size_t ld_dx, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[j] = scale * W[ids[j]], W (vocab, embed) row-major; positions whose id is
+ * pad_idx (negative: none) or outside the table give zeros.                    */
+int nh_embed_fprop(void* out, const void* W, const int32_t* ids, float scale, int dtype, int axis, size_t positions,
+                   size_t embed, size_t vocab, size_t ld_w, size_t ld_out, int64_t pad_idx, void* stream);
+/* dW = beta * dW + scale * G, G[w] = sum of err[j] over the positions with
+ * ids[j] == w, 0 for pad_idx and words that do not occur (beta == 0: dW is not
+ * read; beta == 1: their rows are not touched).  Sums are taken in a fixed order. */
+size_t nh_embed_update_workspace_bytes(int dtype, int axis, size_t positions, size_t embed, size_t vocab);
+int nh_embed_update(void* dW, const void* err, const int32_t* ids, float scale, float beta, int dtype, int axis,
+                    size_t positions, size_t embed, size_t vocab, size_t ld_dw, size_t ld_err, int64_t pad_idx,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Per position: p = softmax of t / temperature over the entries whose id lies
+ * in the vocabulary, q = softmax of z / temperature;
+ *   loss = temperature^2 * sum_k p_k (log p_k - log q[id_k])
+ * stats: four values per position for the backward pass -- the largest z and
+ * log sum_v exp((z_v - largest) / temperature), and the same of the entries' t.
+ * No entry (or only t = -inf): loss 0, largest t -inf.  `strides`, in elements:
+ * ids along entries and positions, t along entries and positions, loss along
+ * positions, stats along its four values and along positions.                  */
+#define NH_DISTILL_MAX_ENTRIES 1024
+size_t nh_distill_workspace_bytes(int backward, int dtype, int axis, size_t vocab, size_t positions, size_t entries);
+int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* ids, const void* t,
+                     float temperature, int dtype, int t_dtype, int axis, size_t vocab, size_t positions, size_t entries,
+                     size_t ld_z, const int64_t* strides, void* workspace, size_t workspace_bytes, void* stream);
+/* dz[v] = weight * temperature * (q[v] - sum of p_k over the entries with id v),
+ * 0 for positions without an entry.  weight[positions], or NULL for weight_all
+ * everywhere.  `strides`: the first four as above, stats along its values and
+ * along positions, weight along positions.  dz must not overlap z.                               */
+int nh_distill_bprop(void* dz, const void* z, const int32_t* ids, const void* t, const float* stats,
+                     const float* weight, float weight_all, float temperature, int dtype, int t_dtype, int axis,
+                     size_t vocab, size_t positions, size_t entries, size_t ld_z, size_t ld_dz, const int64_t* strides,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

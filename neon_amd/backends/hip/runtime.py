@@ -10,7 +10,7 @@ message (hipGetErrorString text or the hiprtc log).
 import ctypes
 import os
 import struct
-from ctypes import (POINTER, byref, c_char, c_char_p, c_float, c_int, c_int32,
+from ctypes import (POINTER, byref, c_char, c_char_p, c_float, c_int, c_int32, c_int64,
                     c_size_t, c_uint8, c_uint16, c_uint32, c_uint64, c_void_p)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -111,6 +111,24 @@ SIGNATURES = {
     "nh_colreduce_workspace_bytes": (c_size_t, [c_uint32, c_uint32]),
     "nh_colmax_argmax_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_uint32, c_uint32,
                                      c_size_t, c_void_p, c_void_p]),
+    "nh_ln_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_size_t, c_size_t]),
+    "nh_ln_fprop": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_int, c_size_t,
+                            c_size_t, c_size_t, c_size_t, c_void_p, c_size_t, c_void_p]),
+    "nh_ln_bprop": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float,
+                            c_int, c_int, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_void_p, c_size_t,
+                            c_void_p]),
+    "nh_embed_fprop": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_int, c_int, c_size_t, c_size_t, c_size_t,
+                               c_size_t, c_size_t, c_int64, c_void_p]),
+    "nh_embed_update_workspace_bytes": (c_size_t, [c_int, c_int, c_size_t, c_size_t, c_size_t]),
+    "nh_embed_update": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_float, c_int, c_int, c_size_t, c_size_t,
+                                c_size_t, c_size_t, c_size_t, c_int64, c_void_p, c_size_t, c_void_p]),
+    "nh_distill_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_size_t, c_size_t, c_size_t]),
+    "nh_distill_fprop": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_int,
+                                 c_int, c_size_t, c_size_t, c_size_t, c_size_t, c_void_p, c_void_p, c_size_t,
+                                 c_void_p]),
+    "nh_distill_bprop": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_float,
+                                 c_int, c_int, c_int, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_void_p,
+                                 c_void_p, c_size_t, c_void_p]),
     "nh_colmax_argmax_f32_static": (c_int, [c_void_p, c_void_p, c_void_p, c_uint32, c_uint32,
                                             c_size_t, c_void_p]),
 }
@@ -141,6 +159,14 @@ def _check(rc):
     if rc != 0:
         msg = _lib.nh_last_error()
         raise HipError(rc, msg.decode("utf-8", "replace") if msg else "unknown error")
+
+
+check = _check      # for callers that use the typed entry points directly
+
+
+def int64s(*values):
+    """a C array of 64-bit integers"""
+    return (c_int64 * len(values))(*values)
 
 
 def device_count():

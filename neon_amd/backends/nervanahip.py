@@ -23,6 +23,7 @@ from neon_amd.backends import backend as _own
 from neon_amd.backends.hip import bf16
 from neon_amd.backends.hip import fastpath
 from neon_amd.backends.hip import runtime as hiprt
+from neon_amd.backends.hip.lmops import LanguageModelOps
 from neon_amd.backends.hip.optree_ir import MixedAxes, Program, REDUCE, eval_const
 from neon_amd.backends.hip import codegen, planner
 from neon_amd.backends.hip.planner import KernelCache, NeedsSplit, make_plan
@@ -544,6 +545,8 @@ class NervanaHIPBase(object):
     as the reference insists: stochastic rounding is requested per tensor
     through its ``rounding`` attribute (mantissa bits, or True for 10).
     """
+    _lm_tensor_base = HIPTensorBase
+
     def __init__(self, rng_seed=None, default_dtype=np.float32, stochastic_round=False,
                  deterministic=None, device_id=0, bench=False, scratch_size=0,
                  hist_bins=64, hist_offset=-48, compat_mode=None, num_devices=None,
@@ -612,6 +615,7 @@ class NervanaHIPBase(object):
         self._rec_coop = None
         self._rec_foreign = False     # the group being recorded made a call that is not a kernel launch
         self._lut_ws = None           # (pointer, bytes) scratch of compound_bprop_lut
+        self._lm_ws = None            # (pointer, bytes) scratch of the language-model operators
         self._originals = frozenset() # ids of handles whose reads mean "before the running group" (compensated_sum)
         self._rec_single = None
         self._temp_pool = {}
@@ -642,6 +646,9 @@ class NervanaHIPBase(object):
             if getattr(self, "_lut_ws", None):
                 rt.free(self._lut_ws[0])
                 self._lut_ws = None
+            if getattr(self, "_lm_ws", None):
+                rt.free(self._lm_ws[0])
+                self._lm_ws = None
         except Exception:
             pass
 
@@ -1660,6 +1667,9 @@ class NervanaHIPBase(object):
         # soon as its last consumer has been enqueued
         self._temp_pool.setdefault((t.shape, t.dtype), []).append(t)
 
+    def _lm_byte_span(self, t):
+        return _byte_span(t)
+
     # -- dense contraction: handed to the library GEMM ---------------------------------------------
     def _gemm_operand(self, t, temps):
         """(tensor, transposed?, leading dimension) for a 2-D operand the GEMM
@@ -2026,7 +2036,12 @@ _COMPOSED_HELPERS = ("fprop_softmax", "fprop_relu", "bprop_relu", "fprop_transfo
                      "compound_rnn_unroll_fprop", "compound_rnn_unroll_bprop")
 for _name in _COMPOSED_HELPERS:
     setattr(NervanaHIPBase, _name, getattr(_own.Backend, _name))
-del _name
+# The language-model operators are written in a module of their own; given to the class in the
+# same way, so that a bound backend class keeps the host's Backend right behind this one.
+for _name, _method in vars(LanguageModelOps).items():
+    if not _name.startswith("__"):
+        setattr(NervanaHIPBase, _name, _method)
+del _name, _method
 
 
 class _Api(object):

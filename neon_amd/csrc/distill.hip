@@ -1,0 +1,542 @@
+// Distillation from a teacher's top logits.  Position n has a student's logits
+// z over the whole vocabulary and K teacher entries (word id, logit t); entries
+// whose id lies outside the vocabulary do not count.  With a temperature T
+//
+//   p = softmax over the entries of t / T        q = softmax over the vocabulary of z / T
+//   loss = T^2 sum_k p_k (log p_k - log q[id_k])
+//   dz_v = w T (q_v - sum of p_k over the entries with id_k == v)
+//
+// A position without entries (or whose t are all -inf) has loss 0 and gradient
+// 0, whatever its logits hold.  Forward reads z once and also leaves what
+// backward starts from: the largest z and the logarithm of the sum of
+// exp((z - largest) / T), and the same of the entries.  (Two numbers each, not
+// their sum: in a log-sum-exp of logits around 1e6 fp32 has no digits left for
+// the logarithm.)  Backward reads z once and writes dz once.  HBM traffic bounds
+// both.
+//
+// Layouts: "rows" (a position's logits lie side by side) and "columns"
+// (positions lie side by side, the backend's usual layout).
+#include "lm_ops.h"
+
+namespace {
+
+using lm::vec;
+
+constexpr int MOST_ENTRIES = NH_DISTILL_MAX_ENTRIES;
+constexpr float LOG2E = 1.44269502f;
+
+struct DistillArgs {
+    const void* z;
+    void* dz;
+    const int32_t* ids;
+    const void* t;
+    float* loss;
+    float* stats;           // four vectors: largest z, log sum, largest t (-inf without entries), log sum
+    long long stat_k;       // from one of them to the next
+    const float* weight;    // nullptr: weight_all
+    float weight_all;
+    float inv_t, temperature;
+    int t_dtype;
+    uint32_t vocab, entries;
+    size_t positions, ld_z, ld_dz;
+    long long ids_k, ids_n, t_k, t_n;           // strides of the entry tensors
+    long long loss_n, stat_n, weight_n;
+    nh_pair* part;          // forward: (maximum, sum) per position and chunk
+    uint2* target;          // backward, columns: (word, probability) per entry and position
+    uint32_t chunk, chunks;
+};
+
+NEON_DEV float load_t(const DistillArgs& a, uint32_t k, size_t n) {
+    const long long at = (long long)k * a.t_k + (long long)n * a.t_n;
+    if (a.t_dtype == NH_T_F32) return ((const float*)a.t)[at];
+    if (a.t_dtype == NH_T_F16) return (float)((const nh_f16*)a.t)[at];
+    return (float)((const nh_bf16*)a.t)[at];
+}
+NEON_DEV int load_id(const DistillArgs& a, uint32_t k, size_t n) {
+    return a.ids[(long long)k * a.ids_k + (long long)n * a.ids_n];
+}
+struct Stats {
+    float top, log_sum, t_top, t_log_sum;
+};
+NEON_DEV Stats load_stats(const DistillArgs& a, size_t n) {
+    const float* p = a.stats + (long long)n * a.stat_n;
+    return {p[0], p[a.stat_k], p[2 * a.stat_k], p[3 * a.stat_k]};
+}
+NEON_DEV float entry_p(const DistillArgs& a, float t, const Stats& s) { return expf((t - s.t_top) * a.inv_t - s.t_log_sum); }
+NEON_DEV bool is_word(int id, uint32_t vocab) { return (uint32_t)id < vocab; }
+
+// (m, s): largest logit seen and sum of e^((z - m) / T).  A state that has seen nothing but
+// -inf keeps s = 0; NaN and +inf make s NaN, as in the two-sweep form.
+struct Lse {
+    float m, s;
+};
+NEON_DEV Lse lse_join(Lse a, Lse b, float c) {
+    Lse r;
+    r.m = nh_max(a.m, b.m);
+    const float z = r.m == -NH_INF ? 0.0f : r.m;
+    r.s = a.s * __builtin_amdgcn_exp2f((a.m - z) * c) + b.s * __builtin_amdgcn_exp2f((b.m - z) * c);
+    return r;
+}
+template <int N> NEON_DEV void lse_add(Lse& a, const float (&x)[N], float c) {
+    float m = a.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = nh_max(m, x[i]);
+    const float z = m == -NH_INF ? 0.0f : m;
+    float s = a.s * __builtin_amdgcn_exp2f((a.m - z) * c);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += __builtin_amdgcn_exp2f((x[i] - z) * c);
+    a.m = m;
+    a.s = s;
+}
+// over the 64 lanes; every lane gets the same bits (the two partners join in lane order)
+NEON_DEV Lse lse_wave(Lse v, float c) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        Lse o;
+        o.m = __shfl_xor(v.m, d);
+        o.s = __shfl_xor(v.s, d);
+        v = (threadIdx.x & d) ? lse_join(o, v, c) : lse_join(v, o, c);
+    }
+    return v;
+}
+NEON_DEV float wave_sum(float v) { return nh_wave_allreduce<nh_op_sum, 64>(v); }
+NEON_DEV float wave_max(float v) { return nh_wave_allreduce<nh_op_max, 64>(v); }
+
+// ---------------------------------------------------------------------------
+// forward: (maximum, sum) of chunks of the vocabulary, then one wave per
+// position joins them in order and adds up the teacher's entries
+// ---------------------------------------------------------------------------
+template <typename T> __global__ __launch_bounds__(256) void distill_rows_lse_kernel(DistillArgs a) {
+    constexpr int V = vec<T>::V, AHEAD = 4;
+    __shared__ Lse slots[4];
+    const size_t n = blockIdx.x / a.chunks;
+    const uint32_t i0 = (blockIdx.x % a.chunks) * a.chunk;
+    const uint32_t i1 = i0 + a.chunk < a.vocab ? i0 + a.chunk : a.vocab;
+    const T* z = (const T*)a.z + n * a.ld_z;
+    const float c = a.inv_t * LOG2E;
+    Lse st = {-NH_INF, 0.0f};
+    uint32_t i = i0 + threadIdx.x * V;
+    for (; i + (AHEAD - 1) * 256 * V + V <= i1; i += AHEAD * 256 * V) {
+        nh_raw<T, V> r[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) r[k].load(z + i + k * 256 * V);
+        float x[AHEAD * V];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[k * V + j] = r[k].get(j);
+        lse_add<AHEAD * V>(st, x, c);
+    }
+    for (; i < i1; i += 256 * V) {
+        nh_raw<T, V> r;
+        const int left = i1 - i < V ? (int)(i1 - i) : V;
+        if (left == V) r.load(z + i);
+        else r.load_partial(z + i, left);
+        float x[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = j < left ? r.get(j) : -NH_INF;
+        lse_add<V>(st, x, c);
+    }
+    st = lse_wave(st, c);
+    if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = st;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        st = lse_join(lse_join(slots[0], slots[1], c), lse_join(slots[2], slots[3], c), c);
+        nh_pair p;
+        p.v = st.m;
+        p.i = __builtin_bit_cast(int, st.s);
+        a.part[(size_t)blockIdx.x] = p;      // [n][chunk]
+    }
+}
+
+constexpr int LC = 8;       // lanes across a strip of 128 bytes of positions
+template <typename T> struct strip { static constexpr int COLS = LC * vec<T>::V; };
+
+template <typename T> __global__ __launch_bounds__(256) void distill_cols_lse_kernel(DistillArgs a) {
+    constexpr int V = vec<T>::V, COLS = strip<T>::COLS, RL = 256 / LC, AHEAD = 8;
+    __shared__ Lse slots[4][COLS];
+    const size_t c0 = (size_t)(blockIdx.x / a.chunks) * COLS;
+    const uint32_t chunk = blockIdx.x % a.chunks;
+    const uint32_t i0 = chunk * a.chunk, i1 = i0 + a.chunk < a.vocab ? i0 + a.chunk : a.vocab;
+    const int cl = threadIdx.x % LC, rl = threadIdx.x / LC;
+    const size_t col = c0 + cl * V;
+    const int n = col >= a.positions ? 0 : (a.positions - col >= V ? V : (int)(a.positions - col));
+    const T* z = (const T*)a.z + col;
+    const float c = a.inv_t * LOG2E;
+    Lse st[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) st[j] = {-NH_INF, 0.0f};
+    if (n > 0)
+        for (uint32_t i = i0 + rl; i < i1; i += AHEAD * RL) {
+            nh_raw<T, V> r[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const uint32_t f = i + k * RL;
+                if (f >= i1) r[k].zero();
+                else if (n == V) r[k].load(z + (size_t)f * a.ld_z);
+                else r[k].load_partial(z + (size_t)f * a.ld_z, n);
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float x[AHEAD];
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) x[k] = i + k * RL < i1 ? r[k].get(j) : -NH_INF;
+                lse_add<AHEAD>(st[j], x, c);
+            }
+        }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+#pragma unroll
+        for (int d = LC; d < 64; d <<= 1) {
+            Lse o;
+            o.m = __shfl_xor(st[j].m, d);
+            o.s = __shfl_xor(st[j].s, d);
+            st[j] = (threadIdx.x & d) ? lse_join(o, st[j], c) : lse_join(st[j], o, c);
+        }
+        if ((threadIdx.x & 63) < LC) slots[threadIdx.x >> 6][cl * V + j] = st[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < COLS && c0 + threadIdx.x < a.positions) {
+        const int x = threadIdx.x;
+        const Lse r = lse_join(lse_join(slots[0][x], slots[1][x], c), lse_join(slots[2][x], slots[3][x], c), c);
+        nh_pair p;
+        p.v = r.m;
+        p.i = __builtin_bit_cast(int, r.s);
+        a.part[(c0 + x) * a.chunks + chunk] = p;
+    }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void distill_finish_kernel(DistillArgs a, size_t z_n, size_t z_v) {
+    const size_t n = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (n >= a.positions) return;
+    const float c = a.inv_t * LOG2E;
+    Lse st = {-NH_INF, 0.0f};
+    for (uint32_t i = lane; i < a.chunks; i += 64) {
+        const nh_pair p = a.part[n * a.chunks + i];
+        st = lse_join(st, {p.v, __builtin_bit_cast(float, p.i)}, c);
+    }
+    st = lse_wave(st, c);
+    const float log_s = logf(st.s);
+
+    float top = -NH_INF;
+    for (uint32_t k = lane; k < a.entries; k += 64)
+        if (is_word(load_id(a, k, n), a.vocab)) top = nh_max(top, load_t(a, k, n));
+    top = wave_max(top);
+    const bool some = top != -NH_INF;
+    const float top0 = some ? top : 0.0f;
+    float sum = 0.0f;
+    for (uint32_t k = lane; k < a.entries; k += 64)
+        if (is_word(load_id(a, k, n), a.vocab)) sum += expf((load_t(a, k, n) - top0) * a.inv_t);
+    sum = wave_sum(sum);
+    const float log_t = logf(sum);
+    float loss = 0.0f;
+    const T* z = (const T*)a.z + n * z_n;
+    for (uint32_t k = lane; k < a.entries && some; k += 64) {
+        const int id = load_id(a, k, n);
+        if (!is_word(id, a.vocab)) continue;
+        const float log_p = (load_t(a, k, n) - top0) * a.inv_t - log_t;
+        const float p = expf(log_p);
+        const float log_q = ((float)z[(size_t)id * z_v] - st.m) * a.inv_t - log_s;
+        if (p != 0.0f) loss = __builtin_fmaf(p, log_p - log_q, loss);
+    }
+    loss = wave_sum(loss);
+    if (lane == 0) {
+        a.loss[(long long)n * a.loss_n] = a.temperature * a.temperature * loss;
+        float* p = a.stats + (long long)n * a.stat_n;
+        p[0] = st.m;
+        p[a.stat_k] = log_s;
+        p[2 * a.stat_k] = top;
+        p[3 * a.stat_k] = log_t;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+NEON_DEV float weight_of(const DistillArgs& a, size_t n) {
+    return (a.weight ? a.weight[(long long)n * a.weight_n] : a.weight_all) * a.temperature;
+}
+NEON_DEV float prob_q(float z, float inv_t, float top, float log_sum) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(z - top, inv_t, -log_sum) * LOG2E);
+}
+
+// One workgroup per position and chunk of the vocabulary: w T q over the chunk,
+// then the few words of the chunk that the teacher names once more with p in.
+template <typename T> __global__ __launch_bounds__(256) void distill_rows_bprop_kernel(DistillArgs a) {
+    constexpr int V = vec<T>::V, AHEAD = 4;
+    __shared__ int ids[MOST_ENTRIES];
+    __shared__ float ps[MOST_ENTRIES];
+    const size_t n = blockIdx.x / a.chunks;
+    const uint32_t i0 = (blockIdx.x % a.chunks) * a.chunk;
+    const uint32_t i1 = i0 + a.chunk < a.vocab ? i0 + a.chunk : a.vocab;
+    const T* z = (const T*)a.z + n * a.ld_z;
+    T* dz = (T*)a.dz + n * a.ld_dz;
+    const Stats st = load_stats(a, n);
+    const bool some = st.t_top != -NH_INF;
+    const float w = weight_of(a, n);
+    for (uint32_t k = threadIdx.x; k < a.entries && some; k += 256) {
+        ids[k] = load_id(a, k, n);
+        ps[k] = entry_p(a, load_t(a, k, n), st);
+    }
+    const auto grad = [&](float x) { return some ? w * prob_q(x, a.inv_t, st.top, st.log_sum) : 0.0f; };
+    uint32_t i = i0 + threadIdx.x * V;
+    for (; i + (AHEAD - 1) * 256 * V + V <= i1; i += AHEAD * 256 * V) {
+        nh_raw<T, V> r[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) r[k].load(z + i + k * 256 * V);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            nh_out<T, V> o;
+            o.clear();
+#pragma unroll
+            for (int j = 0; j < V; ++j) o.set(j, grad(r[k].get(j)));
+            o.store(dz + i + k * 256 * V);
+        }
+    }
+    for (; i < i1; i += 256 * V) {
+        nh_raw<T, V> r;
+        const int left = i1 - i < V ? (int)(i1 - i) : V;
+        if (left == V) r.load(z + i);
+        else r.load_partial(z + i, left);
+        nh_out<T, V> o;
+        o.clear();
+#pragma unroll
+        for (int j = 0; j < V; ++j) o.set(j, grad(r.get(j)));
+        if (left == V) o.store(dz + i);
+        else o.store_partial(dz + i, left);
+    }
+    if (!some) return;
+    __syncthreads();        // the entries are in LDS, and the chunk is written before its words are written again
+    for (uint32_t k = threadIdx.x; k < a.entries; k += 256) {
+        const uint32_t id = (uint32_t)ids[k];
+        if (id < i0 || id >= i1) continue;
+        float p = 0.0f;
+        bool first = true;
+        for (uint32_t o = 0; o < a.entries; ++o)
+            if ((uint32_t)ids[o] == id) {
+                first = first && o >= k;
+                p += ps[o];
+            }
+        if (first) dz[id] = nh_store_cvt<T>::f(w * (prob_q((float)z[id], a.inv_t, st.top, st.log_sum) - p));
+    }
+}
+
+// columns: the teacher's distribution with repeated words joined into their
+// first entry -- (word, probability), word = ~0 for an entry that stands for none
+__global__ __launch_bounds__(64) void distill_target_kernel(DistillArgs a) {
+    __shared__ int ids[MOST_ENTRIES];
+    __shared__ float ps[MOST_ENTRIES];
+    const size_t n = blockIdx.x;
+    const Stats st = load_stats(a, n);
+    const bool some = st.t_top != -NH_INF;
+    for (uint32_t k = threadIdx.x; k < a.entries; k += 64) {
+        ids[k] = some ? load_id(a, k, n) : -1;
+        ps[k] = some ? entry_p(a, load_t(a, k, n), st) : 0.0f;
+    }
+    __syncthreads();
+    for (uint32_t k = threadIdx.x; k < a.entries; k += 64) {
+        const int id = ids[k];
+        bool first = is_word(id, a.vocab);
+        float p = 0.0f;
+        if (first)
+            for (uint32_t o = 0; o < a.entries; ++o)
+                if (ids[o] == id) {
+                    first = first && o >= k;
+                    p += ps[o];
+                }
+        a.target[(size_t)k * a.positions + n] = make_uint2(first ? (uint32_t)id : ~0u, __builtin_bit_cast(uint32_t, p));
+    }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void distill_cols_bprop_kernel(DistillArgs a) {
+    constexpr int V = vec<T>::V, COLS = strip<T>::COLS, RL = 256 / LC, AHEAD = 8;
+    __shared__ float s_top[COLS], s_log[COLS], s_w[COLS];
+    __shared__ bool s_some[COLS];
+    const size_t c0 = (size_t)(blockIdx.x / a.chunks) * COLS;
+    const uint32_t chunk = blockIdx.x % a.chunks;
+    const uint32_t i0 = chunk * a.chunk, i1 = i0 + a.chunk < a.vocab ? i0 + a.chunk : a.vocab;
+    const int cl = threadIdx.x % LC, rl = threadIdx.x / LC;
+    const size_t col = c0 + cl * V;
+    const int n = col >= a.positions ? 0 : (a.positions - col >= V ? V : (int)(a.positions - col));
+    if (threadIdx.x < COLS) {
+        const size_t x = c0 + threadIdx.x;
+        const bool real = x < a.positions;
+        const Stats st = load_stats(a, real ? x : 0);
+        s_top[threadIdx.x] = st.top;
+        s_log[threadIdx.x] = st.log_sum;
+        s_some[threadIdx.x] = real && st.t_top != -NH_INF;
+        s_w[threadIdx.x] = real ? weight_of(a, x) : 0.0f;
+    }
+    __syncthreads();
+    const T* z = (const T*)a.z + col;
+    T* dz = (T*)a.dz + col;
+    float top[V], log_sum[V], w[V];
+    bool some[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        top[j] = s_top[cl * V + j];
+        log_sum[j] = s_log[cl * V + j];
+        w[j] = s_w[cl * V + j];
+        some[j] = s_some[cl * V + j];
+    }
+    if (n > 0)
+        for (uint32_t i = i0 + rl; i < i1; i += AHEAD * RL) {
+            nh_raw<T, V> r[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const uint32_t f = i + k * RL;
+                if (f >= i1) r[k].zero();
+                else if (n == V) r[k].load(z + (size_t)f * a.ld_z);
+                else r[k].load_partial(z + (size_t)f * a.ld_z, n);
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const uint32_t f = i + k * RL;
+                if (f >= i1) continue;
+                nh_out<T, V> o;
+                o.clear();
+#pragma unroll
+                for (int j = 0; j < V; ++j) o.set(j, some[j] ? w[j] * prob_q(r[k].get(j), a.inv_t, top[j], log_sum[j]) : 0.0f);
+                if (n == V) o.store(dz + (size_t)f * a.ld_dz);
+                else o.store_partial(dz + (size_t)f * a.ld_dz, n);
+            }
+        }
+    __syncthreads();
+    const T* z0 = (const T*)a.z + c0;
+    T* dz0 = (T*)a.dz + c0;
+    const uint32_t x = threadIdx.x % COLS;
+    if (c0 + x < a.positions)
+        for (uint32_t k = threadIdx.x / COLS; k < a.entries; k += 256 / COLS) {
+            const uint2 e = a.target[(size_t)k * a.positions + c0 + x];
+            if (e.x < i0 || e.x >= i1) continue;
+            const float q = prob_q((float)z0[(size_t)e.x * a.ld_z + x], a.inv_t, s_top[x], s_log[x]);
+            dz0[(size_t)e.x * a.ld_dz + x] = nh_store_cvt<T>::f(s_w[x] * (q - __builtin_bit_cast(float, e.y)));
+        }
+}
+
+// ---------------------------------------------------------------------------
+// launch geometry: enough workgroups to fill the device, each with enough of
+// the vocabulary to pay for its share of the teacher's entries
+// ---------------------------------------------------------------------------
+struct Chunks {
+    uint32_t len, count;
+};
+Chunks split(size_t vocab, size_t lines, size_t wanted, size_t least) {
+    size_t n = lm::ceil_div(wanted, lines ? lines : 1);
+    const size_t most = lm::ceil_div(vocab, least);
+    if (n > most) n = most;
+    if (n < 1) n = 1;
+    const size_t len = lm::ceil_div(lm::ceil_div(vocab, n), 64) * 64;
+    return {(uint32_t)len, (uint32_t)lm::ceil_div(vocab, len)};
+}
+
+Chunks fprop_chunks(int dtype, int axis, size_t vocab, size_t positions) {
+    if (axis == 1) return split(vocab, positions, 1024, 4096);
+    return split(vocab, lm::ceil_div(positions, (size_t)128 / lm::item_bytes(dtype)), 1024, 256);
+}
+Chunks bprop_chunks(int dtype, int axis, size_t vocab, size_t positions) {
+    if (axis == 1) return split(vocab, positions, 2048, 4096);
+    return split(vocab, lm::ceil_div(positions, (size_t)128 / lm::item_bytes(dtype)), 1024, 256);
+}
+
+size_t workspace_bytes(bool backward, int dtype, int axis, size_t vocab, size_t positions, size_t entries) {
+    if (backward) return axis == 0 ? entries * positions * sizeof(uint2) : 0;
+    return positions * fprop_chunks(dtype, axis, vocab, positions).count * sizeof(nh_pair);
+}
+
+int check(const char* who, int dtype, int t_dtype, int axis, size_t vocab, size_t positions, size_t entries, float temperature,
+          size_t ld_a, size_t ld_b) {
+    if (!lm::known_dtype(dtype) || !lm::known_dtype(t_dtype)) return lm::refuse(who, "unknown storage type");
+    if (axis != 0 && axis != 1) return lm::refuse(who, "axis is 0 or 1");
+    if (vocab == 0 || vocab > 0x7FFFFFFF - 65536) return lm::refuse(who, "between 1 and 2^31 - 65537 words");
+    if (positions > (size_t)1 << 40) return lm::refuse(who, "more than 2^40 positions");
+    if (entries > MOST_ENTRIES) return lm::refuse(who, "more than NH_DISTILL_MAX_ENTRIES entries per position");
+    if (!(temperature > 0.0f) || !(1.0f / temperature > 0.0f) || temperature > NH_FLT_MAX || 1.0f / temperature > NH_FLT_MAX)
+        return lm::refuse(who, "the temperature is a positive finite number");
+    const size_t len = axis == 1 ? vocab : positions, lines = axis == 1 ? positions : vocab;
+    if (lines > 1 && (ld_a < len || ld_b < len)) return lm::refuse(who, "leading dimension shorter than a line");
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t nh_distill_workspace_bytes(int backward, int dtype, int axis, size_t vocab, size_t positions, size_t entries) {
+    if (check("nh_distill_workspace_bytes", dtype, dtype, axis, vocab, positions, entries, 1.0f, axis == 1 ? vocab : positions,
+              axis == 1 ? vocab : positions))
+        return 0;
+    return workspace_bytes(backward != 0, dtype, axis, vocab, positions, entries);
+}
+
+int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* ids, const void* t,
+                     float temperature, int dtype, int t_dtype, int axis, size_t vocab, size_t positions, size_t entries,
+                     size_t ld_z, const int64_t* strides, void* workspace, size_t workspace_bytes_given, void* stream) {
+    const char* who = "nh_distill_fprop";
+    if (int rc = check(who, dtype, t_dtype, axis, vocab, positions, entries, temperature, ld_z, ld_z)) return rc;
+    if (positions == 0) return 0;
+    if (!loss || !stats || !z || !strides || (entries && (!ids || !t))) return lm::refuse(who, "null pointer");
+    const size_t need = workspace_bytes(false, dtype, axis, vocab, positions, entries);
+    if (!workspace || workspace_bytes_given < need) return lm::refuse(who, "workspace smaller than nh_distill_workspace_bytes");
+    if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
+    lm::OnDevice here;
+    const Chunks c = fprop_chunks(dtype, axis, vocab, positions);
+    DistillArgs a = {};
+    a.z = z; a.ids = ids; a.t = t; a.loss = loss; a.stats = stats;
+    a.inv_t = 1.0f / temperature; a.temperature = temperature; a.t_dtype = t_dtype;
+    a.vocab = (uint32_t)vocab; a.entries = (uint32_t)entries; a.positions = positions; a.ld_z = ld_z;
+    a.ids_k = strides[0]; a.ids_n = strides[1]; a.t_k = strides[2]; a.t_n = strides[3]; a.loss_n = strides[4];
+    a.stat_k = strides[5]; a.stat_n = strides[6];
+    a.part = (nh_pair*)workspace; a.chunk = c.len; a.chunks = c.count;
+    return lm::by_dtype(dtype, [&](auto v) {
+        using T = decltype(v);
+        const hipStream_t s = (hipStream_t)stream;
+        const size_t blocks = (axis == 1 ? positions : lm::ceil_div(positions, strip<T>::COLS)) * c.count;
+        if (blocks > lm::MAX_BLOCKS || positions > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
+        if (axis == 1) hipLaunchKernelGGL((distill_rows_lse_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((distill_cols_lse_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((distill_finish_kernel<T>), dim3((unsigned)lm::ceil_div(positions, 4)), dim3(256), 0, s, a,
+                           axis == 1 ? ld_z : (size_t)1, axis == 1 ? (size_t)1 : ld_z);
+        return lm::launched(who);
+    });
+}
+
+int nh_distill_bprop(void* dz, const void* z, const int32_t* ids, const void* t, const float* stats,
+                     const float* weight, float weight_all, float temperature, int dtype, int t_dtype, int axis, size_t vocab,
+                     size_t positions, size_t entries, size_t ld_z, size_t ld_dz, const int64_t* strides, void* workspace,
+                     size_t workspace_bytes_given, void* stream) {
+    const char* who = "nh_distill_bprop";
+    if (int rc = check(who, dtype, t_dtype, axis, vocab, positions, entries, temperature, ld_z, ld_dz)) return rc;
+    if (positions == 0) return 0;
+    if (!dz || !stats || !z || !strides || (entries && (!ids || !t))) return lm::refuse(who, "null pointer");
+    const size_t need = workspace_bytes(true, dtype, axis, vocab, positions, entries);
+    if (need && (!workspace || workspace_bytes_given < need))
+        return lm::refuse(who, "workspace smaller than nh_distill_workspace_bytes");
+    if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
+    lm::OnDevice here;
+    const Chunks c = bprop_chunks(dtype, axis, vocab, positions);
+    DistillArgs a = {};
+    a.z = z; a.dz = dz; a.ids = ids; a.t = t; a.stats = const_cast<float*>(stats);
+    a.weight = weight; a.weight_all = weight_all;
+    a.inv_t = 1.0f / temperature; a.temperature = temperature; a.t_dtype = t_dtype;
+    a.vocab = (uint32_t)vocab; a.entries = (uint32_t)entries; a.positions = positions; a.ld_z = ld_z; a.ld_dz = ld_dz;
+    a.ids_k = strides[0]; a.ids_n = strides[1]; a.t_k = strides[2]; a.t_n = strides[3]; a.stat_k = strides[4];
+    a.stat_n = strides[5]; a.weight_n = strides[6];
+    a.target = (uint2*)workspace; a.chunk = c.len; a.chunks = c.count;
+    return lm::by_dtype(dtype, [&](auto v) {
+        using T = decltype(v);
+        const hipStream_t s = (hipStream_t)stream;
+        const size_t blocks = (axis == 1 ? positions : lm::ceil_div(positions, strip<T>::COLS)) * c.count;
+        if (blocks > lm::MAX_BLOCKS || positions > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
+        if (axis == 1) {
+            hipLaunchKernelGGL((distill_rows_bprop_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+        } else {
+            if (entries) hipLaunchKernelGGL(distill_target_kernel, dim3((unsigned)positions), dim3(64), 0, s, a);
+            hipLaunchKernelGGL((distill_cols_bprop_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+        }
+        return lm::launched(who);
+    });
+}
+
+}  // extern "C"

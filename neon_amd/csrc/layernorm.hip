@@ -33,7 +33,19 @@ struct LnArgs {
     size_t ld_x, ld_dy, ld_out;
 };
 
-NEON_DEV float inv_std(float var, float eps) { return 1.0f / sqrtf(var + eps); }
+// 1 / sqrt(var + eps): the hardware's estimate and one Newton step, within 2
+// units in the last place, in place of a square root and a division (thirty
+// instructions, of which a thread of the column kernels needs eight in a row).
+NEON_DEV float inv_std(float var, float eps) {
+    const float v = var + eps;
+    float r = __builtin_amdgcn_rsqf(v);
+    r = __builtin_fmaf(0.5f * r, __builtin_fmaf(-(v * r), r, 1.0f), r);
+    if (__builtin_expect(!(v >= 1.17549435e-38f && v <= NH_FLT_MAX), 0)) {
+        asm volatile("");                 // (a branch, not a select)
+        r = 1.0f / sqrtf(v);
+    }
+    return r;
+}
 
 // sum over the TPR threads of a row; `slots` (one pair per wave) must not be
 // in use by an earlier call whose readers may not have finished
@@ -373,40 +385,47 @@ template <typename T> __global__ __launch_bounds__(64) void ln_rows_params_kerne
         }
 }
 
-// grads[which][f] = sum of `count` partial rows, in a fixed order: 16 threads
-// per feature take every 16th row, joined in LDS
+// grads[which][f] = sum of `count` partial rows, in a fixed order: 128 threads
+// per 4 features take every 128th row, joined in LDS
 __global__ __launch_bounds__(1024) void ln_param_kernel(LnArgs a, uint32_t count) {
-    __shared__ float join[16][64];
-    const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
-    const size_t f = (size_t)blockIdx.x * 64 + lane;
+    __shared__ float join[128][36];
+    const int lane = threadIdx.x & 7, grp = threadIdx.x >> 3;
+    const uint32_t f = blockIdx.x * 32 + lane * 4;
+    const int n = clip((long long)a.features - f, 4);
     const float* p = a.part + (size_t)blockIdx.y * a.features + f;
-    float s = 0.0f;
-    if (f < a.features)
-        for (uint32_t i = grp; i < count; i += 16) s += p[(size_t)i * 2 * a.features];
-    join[grp][lane] = s;
-    __syncthreads();
-    if (grp == 0 && f < a.features) {
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (n > 0) {
+#pragma unroll 8
+        for (uint32_t i = grp; i < count; i += 128) {
+            float v[4];
+            load_floats<4>(v, p + (size_t)i * 2 * a.features, n);
 #pragma unroll
-        for (int w = 1; w < 16; ++w) s += join[w][lane];
-        a.grads[blockIdx.y][f] = s;
+            for (int k = 0; k < 4; ++k) s[k] += v[k];
+        }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) join[grp][lane * 4 + k] = s[k];
+    __syncthreads();
+    // 32 threads per feature add 4 groups each, then the lanes
+    const int c = threadIdx.x >> 5, part = threadIdx.x & 31;
+    float r = ((join[part][c] + join[part + 32][c]) + join[part + 64][c]) + join[part + 96][c];
+    r = nh_wave_allreduce<nh_op_sum, 32>(r);
+    if (part == 0 && blockIdx.x * 32 + c < a.features) a.grads[blockIdx.y][blockIdx.x * 32 + c] = r;
 }
 
 // ---------------------------------------------------------------------------
-// columns: a workgroup takes a strip of 128 bytes of positions (8 lanes of 16
-// bytes) and NT/8 x RV features at a time.  MODE 0: the strip's features fit
-// one tile, which stays in registers (one read).  MODE 1 leaves the column
-// sums of a run of tiles (blockIdx.y) in the workspace; MODE 2 joins them in
-// order and finishes the same run.
+// columns
 // ---------------------------------------------------------------------------
-constexpr int LC = 8;                 // lanes across a strip
-enum { WHOLE = 0, SUMS = 1, FINISH = 2 };
+// Strips dealt to the XCDs in contiguous runs: the two halves of a cache line
+// that neighbouring strips of 64 bytes read meet in one L2.
+NEON_DEV uint32_t strip_of_block() {
+    const uint32_t n = gridDim.x, b = blockIdx.x, xcd = b % NH_XCDS, rest = n % NH_XCDS;
+    return n < NH_XCDS ? b : xcd * (n / NH_XCDS) + (xcd < rest ? xcd : rest) + b / NH_XCDS;
+}
 
-template <typename T> struct strip { static constexpr int COLS = LC * vec<T>::V; };
-
-// running (count, mean, sum of squared deviations) of two disjoint sets of a column's
-// values joined: with the counts the same for all columns a thread holds, the two factors
-// are computed once
+// Running (mean, sum of squared deviations) of two disjoint sets of a column's
+// values joined: with the counts the same for all columns a thread holds, the two
+// factors are computed once.
 struct JoinFactors {
     float to_b, cross;      // n_b / n and n_a n_b / n
     NEON_DEV JoinFactors(float na, float nb) {
@@ -421,287 +440,457 @@ struct JoinFactors {
     }
 };
 
-template <typename T, int NT, int RV, int MODE>
-__global__ __launch_bounds__(NT) void ln_cols_fprop_kernel(LnArgs a, uint32_t rows_per, uint32_t chunks) {
-    constexpr int V = vec<T>::V, COLS = strip<T>::COLS, NW = NT / 64, RL = NT / LC;
-    __shared__ float s_mean[NW][COLS], s_m2[NW][COLS], s_n[NW];
-    const int t = threadIdx.x, cl = t % LC, rl = t / LC, wave = t >> 6;
-    const size_t c0 = (size_t)blockIdx.x * COLS, c = c0 + cl * V;
-    const int n = clip((long long)a.positions - (long long)c, V);
-    const uint32_t r0 = MODE == WHOLE ? 0 : blockIdx.y * rows_per;
-    const uint32_t r1 = MODE == WHOLE ? a.features : (r0 + rows_per < a.features ? r0 + rows_per : a.features);
-    const T* x = (const T*)a.x + c;
+// Columns, forward: strips of LC lanes of 16 bytes of positions.  A thread holds
+// V neighbouring columns and takes every (NT / LC)-th feature, RV at a time.
+template <typename T, int NT, int LC, int RV> struct ColFprop {
+    static constexpr int V = vec<T>::V, COLS = LC * V, NW = NT / 64, RL = NT / LC;
+    struct Shared {
+        float mean[NW][COLS], m2[NW][COLS], n[NW];
+    };
+    const LnArgs& a;
+    uint32_t strip;
+    int t, cl, rl, n;
+    size_t c0, c;
     nh_raw<T, V> r[RV];
-    float mean[V], m2[V];
+    float g[RV], b[RV];
+    float mean[V], m2[V], count;
 
-    if constexpr (MODE != FINISH) {
+    NEON_DEV ColFprop(const LnArgs& args, uint32_t strip_) : a(args), strip(strip_) {
+        t = threadIdx.x;
+        cl = t % LC;
+        rl = t / LC;
+        c0 = (size_t)strip * COLS;
+        c = c0 + cl * V;
+        n = clip((long long)a.positions - (long long)c, V);
+        count = 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) mean[j] = m2[j] = 0.0f;
-        float cnt = 0.0f;
-        for (uint32_t base = r0; base < r1; base += RL * RV) {
-            int rows = 0;
+    }
+    // features base + rl + i RL below `end` (the last one again behind it)
+    NEON_DEV void load_params(uint32_t base, uint32_t end) {
+#pragma unroll
+        for (int i = 0; i < RV; ++i) {
+            const uint32_t f = base + rl + i * RL < end ? base + rl + i * RL : end - 1;
+            g[i] = a.gamma[f];
+            b[i] = a.beta[f];
+        }
+    }
+    NEON_DEV void load(uint32_t base, uint32_t end) {
+        const T* x = (const T*)a.x + c;
+        if (c0 + COLS <= a.positions) {
 #pragma unroll
             for (int i = 0; i < RV; ++i) {
-                const uint32_t f = base + rl + i * RL;
-                if (f < r1) {
-                    load_clipped(r[i], x + (size_t)f * a.ld_x, n);
-                    ++rows;
-                } else {
-                    r[i].zero();
-                }
+                const uint32_t f = base + rl + i * RL < end ? base + rl + i * RL : end - 1;
+                r[i].load(x + (size_t)f * a.ld_x);
             }
-            const JoinFactors jf(cnt, (float)rows);
-            const float inv = rows > 0 ? 1.0f / (float)rows : 0.0f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < RV; ++i) {
+                const uint32_t f = base + rl + i * RL < end ? base + rl + i * RL : end - 1;
+                load_clipped(r[i], x + (size_t)f * a.ld_x, n);
+            }
+        }
+    }
+    NEON_DEV void add(uint32_t base, uint32_t end) {
+        int rows = 0;
+#pragma unroll
+        for (int i = 0; i < RV; ++i) {
+            if (base + rl + i * RL < end) ++rows;
+            else r[i].zero();
+        }
+        const JoinFactors jf(count, (float)rows);
+        const float inv = rows > 0 ? 1.0f / (float)rows : 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < RV; ++i) s += r[i].get(j);
+            const float m = s * inv;
+            float q = 0.0f;
+#pragma unroll
+            for (int i = 0; i < RV; ++i) {
+                const float d = r[i].get(j) - m;
+                q = __builtin_fmaf(d, i < rows ? d : 0.0f, q);
+            }
+            jf.join(mean[j], m2[j], m, q);
+        }
+        count += (float)rows;
+        // (widened again when they are used next: kept as floats they take twice the registers)
+#pragma unroll
+        for (int i = 0; i < RV; ++i) r[i].keep();
+    }
+    template <int X> NEON_DEV void fold() {
+        if constexpr (X < 64) {
+            const float nb = nh_lane_xor<X>(count);
+            const bool up = (t & X) != 0;
+            // both partners join in the same order, so that they agree to the bit
+            const JoinFactors jf(up ? nb : count, up ? count : nb);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                float s = 0.0f;
-#pragma unroll
-                for (int i = 0; i < RV; ++i) s += r[i].get(j);
-                const float m = s * inv;
-                float q = 0.0f;
-#pragma unroll
-                for (int i = 0; i < RV; ++i) {
-                    const float d = r[i].get(j) - m;
-                    q = __builtin_fmaf(d, i < rows ? d : 0.0f, q);
-                }
-                jf.join(mean[j], m2[j], m, q);
+                const float om = nh_lane_xor<X>(mean[j]), oq = nh_lane_xor<X>(m2[j]);
+                float ma = up ? om : mean[j], qa = up ? oq : m2[j];
+                jf.join(ma, qa, up ? mean[j] : om, up ? m2[j] : oq);
+                mean[j] = ma;
+                m2[j] = qa;
             }
-            cnt += (float)rows;
-            if (MODE == WHOLE) break;
+            count += nb;
+            fold<2 * X>();
         }
-        // lanes of a wave that share columns, then the waves
-        {
-            const auto fold = [&](auto S) {
-                constexpr int X = decltype(S)::value;
-                const float nb = nh_lane_xor<X>(cnt);
-                const bool up = (t & X) != 0;
-                // both partners join in the same order, so that they agree to the bit
-                const JoinFactors jf(up ? nb : cnt, up ? cnt : nb);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float om = nh_lane_xor<X>(mean[j]), oq = nh_lane_xor<X>(m2[j]);
-                    float ma = up ? om : mean[j], qa = up ? oq : m2[j];
-                    jf.join(ma, qa, up ? mean[j] : om, up ? m2[j] : oq);
-                    mean[j] = ma;
-                    m2[j] = qa;
-                }
-                cnt += nb;
-            };
-            fold(std::integral_constant<int, 8>());
-            fold(std::integral_constant<int, 16>());
-            fold(std::integral_constant<int, 32>());
-        }
+    }
+    // lanes of a wave that share columns, then the waves: thread t < COLS gets column t's
+    NEON_DEV float2 join(Shared& m) {
+        fold<LC>();
+        const int wave = t >> 6;
         if ((t & 63) < LC) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                s_mean[wave][cl * V + j] = mean[j];
-                s_m2[wave][cl * V + j] = m2[j];
+                m.mean[wave][cl * V + j] = mean[j];
+                m.m2[wave][cl * V + j] = m2[j];
             }
-            if (cl == 0) s_n[wave] = cnt;
+            if (cl == 0) m.n[wave] = count;
         }
         __syncthreads();
+        float2 r = make_float2(0.0f, 0.0f);
         if (t < COLS) {
-            float m = s_mean[0][t], q = s_m2[0][t], k = s_n[0];
+            r = make_float2(m.mean[0][t], m.m2[0][t]);
+            float k = m.n[0];
             for (int w = 1; w < NW; ++w) {
-                JoinFactors(k, s_n[w]).join(m, q, s_mean[w][t], s_m2[w][t]);
-                k += s_n[w];
-            }
-            if (MODE == SUMS) {
-                float* p = a.part + (((size_t)blockIdx.x * chunks + blockIdx.y) * COLS + t) * 2;
-                p[0] = m;
-                p[1] = q;
-            } else {
-                s_mean[0][t] = m;
-                s_m2[0][t] = q;
+                JoinFactors(k, m.n[w]).join(r.x, r.y, m.mean[w][t], m.m2[w][t]);
+                k += m.n[w];
             }
         }
-    } else {
-        if (t < COLS) {
-            float m = 0.0f, q = 0.0f, k = 0.0f;
-            for (uint32_t i = 0; i < chunks; ++i) {
-                const float* p = a.part + (((size_t)blockIdx.x * chunks + i) * COLS + t) * 2;
-                const uint32_t b = i * rows_per, e = b + rows_per < a.features ? b + rows_per : a.features;
-                JoinFactors(k, (float)(e - b)).join(m, q, p[0], p[1]);
-                k += (float)(e - b);
-            }
-            s_mean[0][t] = m;
-            s_m2[0][t] = q;
-        }
+        return r;
     }
-    if constexpr (MODE != SUMS) {
-        __syncthreads();
+    // thread t < COLS has column t's finished pair: mean and 1 / std for every thread's columns
+    NEON_DEV void share(Shared& m, float2 r, bool keep) {
         const float inv_f = 1.0f / (float)a.features;
-        if (t < COLS && c0 + t < a.positions && (MODE == WHOLE || blockIdx.y == 0)) {
-            a.mean[c0 + t] = s_mean[0][t];
-            a.var[c0 + t] = s_m2[0][t] * inv_f;
+        if (t < COLS) {
+            const float var = r.y * inv_f;
+            m.mean[0][t] = r.x;
+            m.m2[0][t] = inv_std(var, a.eps);
+            if (keep && c0 + t < a.positions) {
+                a.mean[c0 + t] = r.x;
+                a.var[c0 + t] = var;
+            }
         }
-        if (n <= 0) return;
-        float rs[V];
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            mean[j] = s_mean[0][cl * V + j];
-            rs[j] = inv_std(s_m2[0][cl * V + j] * inv_f, a.eps);
+            mean[j] = m.mean[0][cl * V + j];
+            m2[j] = m.m2[0][cl * V + j];
         }
+    }
+    NEON_DEV void put(uint32_t base, uint32_t end) {
         T* y = (T*)a.out + c;
-        for (uint32_t base = r0; base < r1; base += RL * RV) {
-            if constexpr (MODE == FINISH) {
 #pragma unroll
-                for (int i = 0; i < RV; ++i) {
-                    const uint32_t f = base + rl + i * RL;
-                    if (f < r1) load_clipped(r[i], x + (size_t)f * a.ld_x, n);
-                }
-            }
+        for (int i = 0; i < RV; ++i) {
+            const uint32_t f = base + rl + i * RL;
+            if (f >= end) continue;
+            nh_out<T, V> o;
+            o.clear();
 #pragma unroll
-            for (int i = 0; i < RV; ++i) {
-                const uint32_t f = base + rl + i * RL;
-                if (f >= r1) continue;
-                const float g = a.gamma[f], b = a.beta[f];
-                nh_out<T, V> o;
-                o.clear();
-#pragma unroll
-                for (int j = 0; j < V; ++j) o.set(j, __builtin_fmaf((r[i].get(j) - mean[j]) * rs[j], g, b));
-                store_clipped(o, y + (size_t)f * a.ld_out, n);
-            }
-            if (MODE == WHOLE) break;
+            for (int j = 0; j < V; ++j) o.set(j, __builtin_fmaf((r[i].get(j) - mean[j]) * m2[j], g[i], b[i]));
+            store_clipped(o, y + (size_t)f * a.ld_out, n);
         }
+    }
+};
+
+// The features of a strip in registers: x is read once.  Loads return in the
+// order of issue, stores among them, so gamma and beta are asked for first.
+template <typename T, int NT, int LC, int RV> __global__ __launch_bounds__(NT, 4) void ln_cols_fprop_kernel(LnArgs a) {
+    using K = ColFprop<T, NT, LC, RV>;
+    __shared__ typename K::Shared m;
+    K k(a, strip_of_block());
+    k.load_params(0, a.features);
+    k.load(0, a.features);
+    k.add(0, a.features);
+    k.share(m, k.join(m), true);
+    k.put(0, a.features);
+}
+
+// More features than that: statistics of runs of features (blockIdx.y), then the
+// runs' statistics joined in order by every workgroup that finishes one.
+template <typename T> __global__ __launch_bounds__(256) void ln_cols_fprop_sums_kernel(LnArgs a, uint32_t rows_per, uint32_t chunks,
+                                                                                      float2* sums) {
+    using K = ColFprop<T, 256, 8, 8>;
+    __shared__ typename K::Shared m;
+    K k(a, strip_of_block());
+    const uint32_t r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < a.features ? r0 + rows_per : a.features;
+    for (uint32_t base = r0; base < r1; base += K::RL * 8) {
+        k.load(base, r1);
+        k.add(base, r1);
+    }
+    const float2 r = k.join(m);
+    if (k.t < K::COLS) sums[((size_t)k.strip * chunks + blockIdx.y) * K::COLS + k.t] = r;
+}
+template <typename T> __global__ __launch_bounds__(256) void ln_cols_fprop_finish_kernel(LnArgs a, uint32_t rows_per, uint32_t chunks,
+                                                                                        const float2* sums) {
+    using K = ColFprop<T, 256, 8, 8>;
+    __shared__ typename K::Shared m;
+    K k(a, strip_of_block());
+    const uint32_t r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < a.features ? r0 + rows_per : a.features;
+    k.load_params(r0, r1);
+    k.load(r0, r1);
+    float2 r = make_float2(0.0f, 0.0f);
+    if (k.t < K::COLS) {
+        float seen = 0.0f;
+        for (uint32_t i = 0; i < chunks; ++i) {
+            const float2 p = sums[((size_t)k.strip * chunks + i) * K::COLS + k.t];
+            const uint32_t b = i * rows_per, e = b + rows_per < a.features ? b + rows_per : a.features;
+            JoinFactors(seen, (float)(e - b)).join(r.x, r.y, p.x, p.y);
+            seen += (float)(e - b);
+        }
+    }
+    k.share(m, r, blockIdx.y == 0);
+    for (uint32_t base = r0; base < r1; base += K::RL * 8) {
+        if (base != r0) {
+            k.load_params(base, r1);
+            k.load(base, r1);
+        }
+        k.put(base, r1);
     }
 }
 
-template <typename T, int NT, int RV, int MODE>
-__global__ __launch_bounds__(NT) void ln_cols_bprop_kernel(LnArgs a, uint32_t rows_per, uint32_t chunks, float* sums) {
-    constexpr int V = vec<T>::V, COLS = strip<T>::COLS, NW = NT / 64, RL = NT / LC;
-    __shared__ float s_a[NW][COLS], s_b[NW][COLS];
-    const int t = threadIdx.x, cl = t % LC, rl = t / LC, wave = t >> 6;
-    const size_t c0 = (size_t)blockIdx.x * COLS, c = c0 + cl * V;
-    const int n = clip((long long)a.positions - (long long)c, V);
-    const uint32_t r0 = MODE == WHOLE ? 0 : blockIdx.y * rows_per;
-    const uint32_t r1 = MODE == WHOLE ? a.features : (r0 + rows_per < a.features ? r0 + rows_per : a.features);
-    const T* x = (const T*)a.x + c;
-    const T* dy = (const T*)a.dy + c;
-    nh_raw<T, V> rx[RV], rd[RV];
-    float mu[V], rs[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        mu[j] = j < n ? a.mean[c + j] : 0.0f;
-        rs[j] = j < n ? inv_std(a.var[c + j], a.eps) : 0.0f;
-    }
-    if constexpr (MODE != FINISH) {
-        float s1[V], s2[V];
+// Columns, backward: strips of 64 bytes of positions (4 lanes of 16 bytes).  A
+// thread holds V neighbouring columns and takes every (NT / 4)-th feature.
+constexpr int BLC = 4;
+template <typename T> struct bstrip { static constexpr int COLS = BLC * vec<T>::V; };
+
+template <typename T, int NT> struct ColBprop {
+    static constexpr int V = vec<T>::V, COLS = bstrip<T>::COLS, NW = NT / 64, RL = NT / BLC;
+    struct Shared {
+        float a[NW][COLS], b[NW][COLS];
+    };
+    const LnArgs& a;
+    uint32_t strip;
+    int t, cl, rl, n;
+    size_t c0, c;
+    const T* x;
+    const T* dy;
+    float mu[V], rs[V], s1[V], s2[V];
+
+    NEON_DEV ColBprop(const LnArgs& args, uint32_t strip_) : a(args), strip(strip_) {
+        t = threadIdx.x;
+        cl = t % BLC;
+        rl = t / BLC;
+        c0 = (size_t)strip * COLS;
+        c = c0 + cl * V;
+        n = clip((long long)a.positions - (long long)c, V);
+        x = (const T*)a.x + c;
+        dy = (const T*)a.dy + c;
 #pragma unroll
         for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
-        float* part = a.part + (size_t)blockIdx.x * 2 * a.features;
-        for (uint32_t base = r0; base < r1; base += RL * RV) {
-#pragma unroll
-            for (int i = 0; i < RV; ++i) {
-                const uint32_t f = base + rl + i * RL;
-                const int m = f < r1 ? n : 0;
-                load_clipped(rx[i], x + (size_t)f * a.ld_x, m);
-                load_clipped(rd[i], dy + (size_t)f * a.ld_dy, m);
-            }
-#pragma unroll
-            for (int i = 0; i < RV; ++i) {
-                const uint32_t f = base + rl + i * RL;
-                const float g = f < r1 ? a.gamma[f] : 0.0f;
-                float dg = 0.0f, db = 0.0f;
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float h = (rx[i].get(j) - mu[j]) * rs[j], d = rd[i].get(j), u = d * g;
-                    s1[j] += u;
-                    s2[j] = __builtin_fmaf(u, h, s2[j]);
-                    dg = __builtin_fmaf(d, h, dg);
-                    db += d;
-                }
-                dg = nh_wave_allreduce<nh_op_sum, LC>(dg);
-                db = nh_wave_allreduce<nh_op_sum, LC>(db);
-                if (cl == 0 && f < r1) {
-                    part[f] = dg;
-                    part[a.features + f] = db;
-                }
-            }
-            if (MODE == WHOLE) break;
-        }
+    }
+    NEON_DEV void load_stats() {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            s1[j] += nh_lane_xor<8>(s1[j]);
-            s2[j] += nh_lane_xor<8>(s2[j]);
-            s1[j] += nh_lane_xor<16>(s1[j]);
-            s2[j] += nh_lane_xor<16>(s2[j]);
-            s1[j] += nh_lane_xor<32>(s1[j]);
-            s2[j] += nh_lane_xor<32>(s2[j]);
-        }
-        if ((t & 63) < LC) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                s_a[wave][cl * V + j] = s1[j];
-                s_b[wave][cl * V + j] = s2[j];
-            }
-        }
-        __syncthreads();
-        if (t < COLS) {
-            float p = s_a[0][t], q = s_b[0][t];
-            for (int w = 1; w < NW; ++w) {
-                p += s_a[w][t];
-                q += s_b[w][t];
-            }
-            if (MODE == SUMS) {
-                float* o = sums + (((size_t)blockIdx.x * chunks + blockIdx.y) * COLS + t) * 2;
-                o[0] = p;
-                o[1] = q;
-            } else {
-                s_a[0][t] = p;
-                s_b[0][t] = q;
-            }
-        }
-    } else {
-        if (t < COLS) {
-            float p = 0.0f, q = 0.0f;
-            for (uint32_t i = 0; i < chunks; ++i) {
-                const float* o = sums + (((size_t)blockIdx.x * chunks + i) * COLS + t) * 2;
-                p += o[0];
-                q += o[1];
-            }
-            s_a[0][t] = p;
-            s_b[0][t] = q;
+            mu[j] = j < n ? a.mean[c + j] : 0.0f;
+            rs[j] = j < n ? inv_std(a.var[c + j], a.eps) : 0.0f;
         }
     }
-    if constexpr (MODE != SUMS) {
-        __syncthreads();
-        if (n <= 0) return;
-        const float inv_f = 1.0f / (float)a.features;
-        float s1[V], s2[V];
+    // one feature's share of the column sums; returns the feature's sums over the strip
+    NEON_DEV float2 add(const nh_raw<T, V>& rx, const nh_raw<T, V>& rd, float g) {
+        float dg = 0.0f, db = 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            s1[j] = s_a[0][cl * V + j] * inv_f;
-            s2[j] = s_b[0][cl * V + j] * inv_f;
+            const float d = rd.get(j), e = (rx.get(j) - mu[j]) * d;
+            s1[j] = __builtin_fmaf(d, g, s1[j]);
+            s2[j] = __builtin_fmaf(e, g, s2[j]);           // without the column's factor 1 / std, which share() adds
+            dg = __builtin_fmaf(e, rs[j], dg);
+            db += d;
         }
-        T* dx = (T*)a.out + c;
-        for (uint32_t base = r0; base < r1; base += RL * RV) {
-            if constexpr (MODE == FINISH) {
+        // (the sums are in registers here: left to itself the compiler puts these additions off until
+        // they are read, and keeps every h and d for them)
+#pragma unroll
+        for (int j = 0; j < V; ++j) asm volatile("" : "+v"(s1[j]), "+v"(s2[j]));
+        return make_float2(nh_wave_allreduce<nh_op_sum, BLC>(dg), nh_wave_allreduce<nh_op_sum, BLC>(db));
+    }
+    NEON_DEV void put_sums(uint32_t f, float2 r) {
+        float* part = a.part + (size_t)strip * 2 * a.features;
+        part[f] = r.x;
+        part[a.features + f] = r.y;
+    }
+    NEON_DEV void put(const nh_raw<T, V>& rx, const nh_raw<T, V>& rd, float g, uint32_t f) {
+        nh_out<T, V> o;
+        o.clear();
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            // s1, s2 as share() leaves them: r mean(u), r^2 mean(u h)
+            const float u = __builtin_fmaf(rd.get(j) * rs[j], g, -s1[j]);
+            o.set(j, __builtin_fmaf(-s2[j], rx.get(j) - mu[j], u));
+        }
+        store_clipped(o, (T*)a.out + c + (size_t)f * a.ld_out, n);
+    }
+    // features [r0, r1) straight from memory, a few at a time
+    template <int RV, class F> NEON_DEV void stream(uint32_t r0, uint32_t r1, F each) {
+        const bool full = c0 + COLS <= a.positions;
+        for (uint32_t base = r0 + rl; base - rl < r1; base += RL * RV) {
+            nh_raw<T, V> rx[RV], rd[RV];
+            float g[RV];
+#pragma unroll
+            for (int i = 0; i < RV; ++i) g[i] = a.gamma[base + i * RL < r1 ? base + i * RL : r1 - 1];
+            if (full) {
 #pragma unroll
                 for (int i = 0; i < RV; ++i) {
-                    const uint32_t f = base + rl + i * RL;
-                    const int m = f < r1 ? n : 0;
-                    load_clipped(rx[i], x + (size_t)f * a.ld_x, m);
-                    load_clipped(rd[i], dy + (size_t)f * a.ld_dy, m);
+                    const uint32_t f = base + i * RL < r1 ? base + i * RL : r1 - 1;
+                    rx[i].load(x + (size_t)f * a.ld_x);
+                    rd[i].load(dy + (size_t)f * a.ld_dy);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < RV; ++i) {
+                    const uint32_t f = base + i * RL < r1 ? base + i * RL : r1 - 1;
+                    load_clipped(rx[i], x + (size_t)f * a.ld_x, n);
+                    load_clipped(rd[i], dy + (size_t)f * a.ld_dy, n);
                 }
             }
 #pragma unroll
             for (int i = 0; i < RV; ++i) {
-                const uint32_t f = base + rl + i * RL;
-                if (f >= r1) continue;
-                const float g = a.gamma[f];
-                nh_out<T, V> o;
-                o.clear();
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float h = (rx[i].get(j) - mu[j]) * rs[j], u = rd[i].get(j) * g;
-                    o.set(j, rs[j] * ((u - s1[j]) - h * s2[j]));
+                const uint32_t f = base + i * RL;
+                if (f >= r1) {       // (a feature once more: no error, no share)
+                    rx[i].zero();
+                    rd[i].zero();
                 }
-                store_clipped(o, dx + (size_t)f * a.ld_out, n);
+                each(rx[i], rd[i], g[i], f, f < r1);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (MODE == WHOLE) break;
         }
     }
+    // column sums over the 16 lanes of a wave that share columns and over the waves:
+    // thread t < COLS gets column t's
+    NEON_DEV float2 join(Shared& m) {
+        const int j = nh_col_wave_fold<nh_op_sum, V, BLC>(s1);
+        nh_col_wave_fold<nh_op_sum, V, BLC>(s2);
+        constexpr int LEFT = V * BLC / 64 > 1 ? V * BLC / 64 : 1;      // columns a lane is left with
+#pragma unroll
+        for (int i = 0; i < LEFT; ++i) {
+            m.a[t >> 6][cl * V + j + i] = s1[i];
+            m.b[t >> 6][cl * V + j + i] = s2[i];
+        }
+        __syncthreads();
+        float2 r = make_float2(0.0f, 0.0f);
+        if (t < COLS)
+            for (int w = 0; w < NW; ++w) {
+                r.x += m.a[w][t];
+                r.y += m.b[w][t];
+            }
+        return r;
+    }
+    // thread t < COLS has the finished sums of column t: means for every thread's columns
+    NEON_DEV void share(Shared& m, float2 r) {
+        const float inv_f = 1.0f / (float)a.features;
+        if (t < COLS) {
+            m.a[0][t] = r.x * inv_f;
+            m.b[0][t] = r.y * inv_f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            s1[j] = m.a[0][cl * V + j] * rs[j];
+            s2[j] = m.b[0][cl * V + j] * rs[j] * rs[j] * rs[j];
+        }
+    }
+};
+
+// The features of a strip in registers (RV per thread): x and dy are read once.
+// The strip that the positions end in streams them twice instead.
+//
+// Loads return in the order of issue, stores among them: what is small (the
+// statistics, gamma) is asked for first, the features' sums go through LDS and
+// are stored last, so that the additions of a feature wait for its own two loads
+// only.
+template <typename T, int NT, int RV> __global__ __launch_bounds__(NT, 4) void ln_cols_bprop_kernel(LnArgs a) {
+    using K = ColBprop<T, NT>;
+    __shared__ typename K::Shared m;
+    __shared__ float2 feature[K::RL * RV];
+    K k(a, strip_of_block());
+    const uint32_t last = a.features - 1;
+    if (k.c0 + K::COLS <= a.positions) {
+        k.load_stats();
+        nh_raw<T, K::V> rx[RV], rd[RV];
+        float g[RV];
+#pragma unroll
+        for (int i = 0; i < RV; ++i) {
+            const uint32_t f = k.rl + i * K::RL;
+            g[i] = a.gamma[f < last ? f : last];
+        }
+#pragma unroll
+        for (int i = 0; i < RV; ++i) {
+            const uint32_t f = k.rl + i * K::RL < last ? k.rl + i * K::RL : last;
+            rx[i].load(k.x + (size_t)f * a.ld_x);
+            rd[i].load(k.dy + (size_t)f * a.ld_dy);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < RV; ++i) {
+            const uint32_t f = k.rl + i * K::RL;
+            if (f > last) {       // (a feature once more: no error, no share)
+                rx[i].zero();
+                rd[i].zero();
+            }
+            const float2 r = k.add(rx[i], rd[i], g[i]);
+            if (k.cl == 0) feature[f] = r;
+            // the packed values are widened again below: kept as floats, or with the rows
+            // interleaved, two tensors do not fit 128 registers
+            rx[i].keep();
+            rd[i].keep();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        k.share(m, k.join(m));
+#pragma unroll
+        for (int i = 0; i < RV; ++i) {
+            const uint32_t f = k.rl + i * K::RL;
+            if (f <= last) k.put(rx[i], rd[i], g[i], f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+        k.load_stats();
+        k.template stream<2>(0, a.features, [&](const auto& rx, const auto& rd, float g, uint32_t f, bool on) {
+            const float2 r = k.add(rx, rd, g);
+            if (k.cl == 0 && on) feature[f] = r;
+        });
+        k.share(m, k.join(m));
+        k.template stream<2>(0, a.features, [&](const auto& rx, const auto& rd, float g, uint32_t f, bool on) {
+            if (on) k.put(rx, rd, g, f);
+        });
+    }
+    for (uint32_t f = threadIdx.x; f <= last; f += NT) k.put_sums(f, feature[f]);
+}
+
+// More features than that: column sums of runs of features (blockIdx.y), then
+// the runs' sums joined in order by every workgroup that finishes one.
+template <typename T> __global__ __launch_bounds__(256) void ln_cols_bprop_sums_kernel(LnArgs a, uint32_t rows_per, uint32_t chunks,
+                                                                                      float2* sums) {
+    using K = ColBprop<T, 256>;
+    __shared__ typename K::Shared m;
+    K k(a, strip_of_block());
+    const uint32_t r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < a.features ? r0 + rows_per : a.features;
+    k.load_stats();
+    k.template stream<2>(r0, r1, [&](const auto& rx, const auto& rd, float g, uint32_t f, bool on) {
+        const float2 r = k.add(rx, rd, g);
+        if (k.cl == 0 && on) k.put_sums(f, r);
+    });
+    const float2 r = k.join(m);
+    if (k.t < K::COLS) sums[((size_t)k.strip * chunks + blockIdx.y) * K::COLS + k.t] = r;
+}
+template <typename T> __global__ __launch_bounds__(256) void ln_cols_bprop_finish_kernel(LnArgs a, uint32_t rows_per, uint32_t chunks,
+                                                                                        const float2* sums) {
+    using K = ColBprop<T, 256>;
+    __shared__ typename K::Shared m;
+    K k(a, strip_of_block());
+    const uint32_t r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < a.features ? r0 + rows_per : a.features;
+    k.load_stats();
+    float2 r = make_float2(0.0f, 0.0f);
+    if (k.t < K::COLS)
+        for (uint32_t i = 0; i < chunks; ++i) {
+            const float2 p = sums[((size_t)k.strip * chunks + i) * K::COLS + k.t];
+            r.x += p.x;
+            r.y += p.y;
+        }
+    k.share(m, r);
+    k.template stream<2>(r0, r1, [&](const auto& rx, const auto& rd, float g, uint32_t f, bool on) {
+        if (on) k.put(rx, rd, g, f);
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -711,43 +900,47 @@ constexpr size_t LONG_ROW_FPROP = 65536;      // features one workgroup's regist
 constexpr size_t LONG_ROW_BPROP = 16384;
 constexpr unsigned ROW_GROUPS = 512;          // workgroups that walk the rows in the backward pass
 constexpr unsigned LONG_ROW_RUNS = 64;        // row runs per feature strip in ln_rows_params_kernel
-constexpr size_t COL_TILE = 256;              // features per tile of the split column kernels
-constexpr size_t COL_RESIDENT = 1024;         // features a 1024-thread workgroup keeps
-constexpr size_t COL_CHUNKS = 32;             // runs of tiles per strip, at most
+constexpr size_t COL_CHUNKS = 32;             // runs of tiles per strip of a split column kernel, at most
 
-size_t strip_cols(int dtype) { return (size_t)128 / lm::item_bytes(dtype); }
+// forward and backward column kernels: features of one tile of the split form, features that stay in registers
+struct ColLimits {
+    size_t tile, resident, bytes;             // bytes: width of a strip
+};
+constexpr ColLimits COL_FPROP = {256, 2048, 128}, COL_BPROP = {512, 2048, 64};
+
+size_t strips_of(const ColLimits& l, int dtype, size_t positions) { return lm::ceil_div(positions, l.bytes / lm::item_bytes(dtype)); }
 
 struct ColSplit {
     uint32_t rows_per, chunks;
 };
-ColSplit split_columns(size_t features) {
-    const size_t tiles = lm::ceil_div(features, COL_TILE);
+ColSplit split_columns(const ColLimits& l, size_t features) {
+    const size_t tiles = lm::ceil_div(features, l.tile);
     const size_t per = lm::ceil_div(tiles, COL_CHUNKS);
-    return {(uint32_t)(per * COL_TILE), (uint32_t)lm::ceil_div(tiles, per)};
+    return {(uint32_t)(per * l.tile), (uint32_t)lm::ceil_div(tiles, per)};
 }
 
-unsigned row_groups(size_t features, size_t positions, int dtype) {
+unsigned row_groups(size_t features, size_t positions) {
     const size_t per_block = features <= (size_t)64 * 16 ? 4 : 1;
     const size_t blocks = lm::ceil_div(positions, per_block);
     return (unsigned)(blocks < ROW_GROUPS ? blocks : ROW_GROUPS);
 }
 
 size_t partial_rows(size_t features, size_t positions, int dtype, bool columns) {
-    if (columns) return lm::ceil_div(positions, strip_cols(dtype));
+    if (columns) return strips_of(COL_BPROP, dtype, positions);
     if (features > LONG_ROW_BPROP) return positions < LONG_ROW_RUNS ? positions : LONG_ROW_RUNS;
-    return row_groups(features, positions, dtype);
+    return row_groups(features, positions);
 }
 
-size_t column_sum_bytes(size_t features, size_t positions, int dtype) {
-    return lm::align256(lm::ceil_div(positions, strip_cols(dtype)) * split_columns(features).chunks * strip_cols(dtype) * 2 *
-                        sizeof(float));
+size_t column_sum_bytes(const ColLimits& l, size_t features, size_t positions, int dtype) {
+    if (features <= l.resident) return 0;
+    return lm::align256(strips_of(l, dtype, positions) * split_columns(l, features).chunks * (l.bytes / lm::item_bytes(dtype)) *
+                        2 * sizeof(float));
 }
 
 size_t workspace_bytes(bool backward, int dtype, bool columns, size_t features, size_t positions) {
-    size_t need = 0;
-    if (columns && features > COL_RESIDENT) need += column_sum_bytes(features, positions, dtype);
-    if (backward) need += lm::align256(partial_rows(features, positions, dtype, columns) * 2 * features * sizeof(float));
-    return need;
+    if (!backward) return columns ? column_sum_bytes(COL_FPROP, features, positions, dtype) : 0;
+    return (columns ? column_sum_bytes(COL_BPROP, features, positions, dtype) : 0) +
+           lm::align256(partial_rows(features, positions, dtype, columns) * 2 * features * sizeof(float));
 }
 
 int check(const char* who, int dtype, int axis, size_t features, size_t positions, size_t ld_min_a, size_t ld_min_b,
@@ -761,6 +954,8 @@ int check(const char* who, int dtype, int axis, size_t features, size_t position
         return lm::refuse(who, "leading dimension shorter than a line");
     return 0;
 }
+
+template <typename T> constexpr int code_of() { return sizeof(T) == 4 ? NH_T_F32 : NH_T_F16; }     // (as far as sizes go)
 
 template <typename T> int fprop_rows(const LnArgs& a, hipStream_t s) {
     constexpr size_t V = vec<T>::V;
@@ -783,29 +978,37 @@ template <typename T> int fprop_rows(const LnArgs& a, hipStream_t s) {
 }
 
 template <typename T> int fprop_cols(const LnArgs& a, hipStream_t s) {
-    const size_t strips = lm::ceil_div(a.positions, strip<T>::COLS);
-    if (strips > lm::MAX_BLOCKS) return lm::refuse("nh_ln_fprop", "too many positions for one launch");
-    if (a.features <= COL_TILE) {
-        hipLaunchKernelGGL((ln_cols_fprop_kernel<T, 256, 8, WHOLE>), dim3((unsigned)strips), dim3(256), 0, s, a, 0u, 1u);
-    } else if (a.features <= COL_RESIDENT) {
-        hipLaunchKernelGGL((ln_cols_fprop_kernel<T, 1024, 8, WHOLE>), dim3((unsigned)strips), dim3(1024), 0, s, a, 0u, 1u);
+    const size_t wide = strips_of(COL_FPROP, code_of<T>(), a.positions);
+    if (4 * wide > lm::MAX_BLOCKS) return lm::refuse("nh_ln_fprop", "too many positions for one launch");
+#define LN_GO(NT, LC) hipLaunchKernelGGL((ln_cols_fprop_kernel<T, NT, LC, 8>), dim3((unsigned)lm::ceil_div(a.positions, (LC) * vec<T>::V)), dim3(NT), 0, s, a)
+    const bool many = wide >= 512;
+    if (a.features <= COL_FPROP.tile) {
+        if (many) LN_GO(256, 8);
+        else LN_GO(256, 4);
+    } else if (a.features <= 1024) {
+        if (many) LN_GO(1024, 8);
+        else LN_GO(512, 4);
+    } else if (a.features <= COL_FPROP.resident) {
+        LN_GO(1024, 4);
     } else {
-        const ColSplit c = split_columns(a.features);
-        const dim3 grid((unsigned)strips, c.chunks);
-        hipLaunchKernelGGL((ln_cols_fprop_kernel<T, 256, 8, SUMS>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks);
-        hipLaunchKernelGGL((ln_cols_fprop_kernel<T, 256, 8, FINISH>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks);
+        const ColSplit c = split_columns(COL_FPROP, a.features);
+        const dim3 grid((unsigned)wide, c.chunks);
+        float2* sums = (float2*)a.part;
+        hipLaunchKernelGGL((ln_cols_fprop_sums_kernel<T>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks, sums);
+        hipLaunchKernelGGL((ln_cols_fprop_finish_kernel<T>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks, (const float2*)sums);
     }
+#undef LN_GO
     return lm::launched("nh_ln_fprop");
 }
 
 void add_params(const LnArgs& a, size_t count, hipStream_t s) {
-    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)lm::ceil_div(a.features, 64), 2), dim3(1024), 0, s, a, (uint32_t)count);
+    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)lm::ceil_div(a.features, 32), 2), dim3(1024), 0, s, a, (uint32_t)count);
 }
 
 template <typename T> int bprop_rows(const LnArgs& a, hipStream_t s) {
     constexpr size_t V = vec<T>::V;
     const size_t nvec = lm::ceil_div(a.features, V);
-    const size_t rows = partial_rows(a.features, a.positions, sizeof(T) == 4 ? NH_T_F32 : NH_T_F16, false);
+    const size_t rows = partial_rows(a.features, a.positions, code_of<T>(), false);
     if (a.features > LONG_ROW_BPROP) {
         if (a.positions > lm::MAX_BLOCKS) return lm::refuse("nh_ln_bprop", "too many positions for one launch");
         const size_t per = lm::ceil_div(a.positions, rows);
@@ -830,21 +1033,22 @@ template <typename T> int bprop_rows(const LnArgs& a, hipStream_t s) {
 }
 
 template <typename T> int bprop_cols(LnArgs a, char* ws, hipStream_t s) {
-    const size_t strips = lm::ceil_div(a.positions, strip<T>::COLS);
+    const size_t strips = strips_of(COL_BPROP, code_of<T>(), a.positions);
     if (strips > lm::MAX_BLOCKS) return lm::refuse("nh_ln_bprop", "too many positions for one launch");
-    if (a.features <= COL_TILE) {
-        a.part = (float*)ws;
-        hipLaunchKernelGGL((ln_cols_bprop_kernel<T, 256, 8, WHOLE>), dim3((unsigned)strips), dim3(256), 0, s, a, 0u, 1u, nullptr);
-    } else if (a.features <= COL_RESIDENT) {
-        a.part = (float*)ws;
-        hipLaunchKernelGGL((ln_cols_bprop_kernel<T, 1024, 8, WHOLE>), dim3((unsigned)strips), dim3(1024), 0, s, a, 0u, 1u, nullptr);
+    float2* sums = (float2*)ws;
+    a.part = (float*)(ws + column_sum_bytes(COL_BPROP, a.features, a.positions, code_of<T>()));
+    const dim3 whole((unsigned)strips);
+    if (a.features <= 512) {
+        hipLaunchKernelGGL((ln_cols_bprop_kernel<T, 256, 8>), whole, dim3(256), 0, s, a);
+    } else if (a.features <= 1024) {
+        hipLaunchKernelGGL((ln_cols_bprop_kernel<T, 512, 8>), whole, dim3(512), 0, s, a);
+    } else if (a.features <= COL_BPROP.resident) {
+        hipLaunchKernelGGL((ln_cols_bprop_kernel<T, 1024, 8>), whole, dim3(1024), 0, s, a);
     } else {
-        const ColSplit c = split_columns(a.features);
+        const ColSplit c = split_columns(COL_BPROP, a.features);
         const dim3 grid((unsigned)strips, c.chunks);
-        float* sums = (float*)ws;
-        a.part = (float*)(ws + column_sum_bytes(a.features, a.positions, sizeof(T) == 4 ? NH_T_F32 : NH_T_F16));
-        hipLaunchKernelGGL((ln_cols_bprop_kernel<T, 256, 8, SUMS>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks, sums);
-        hipLaunchKernelGGL((ln_cols_bprop_kernel<T, 256, 8, FINISH>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks, sums);
+        hipLaunchKernelGGL((ln_cols_bprop_sums_kernel<T>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks, sums);
+        hipLaunchKernelGGL((ln_cols_bprop_finish_kernel<T>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks, (const float2*)sums);
     }
     add_params(a, strips, s);
     return lm::launched("nh_ln_bprop");

@@ -31,6 +31,7 @@ struct LnArgs {
     uint32_t features;
     size_t positions;
     size_t ld_x, ld_dy, ld_out;
+    bool stream;          // the output is larger than what the caches keep of it
 };
 
 // 1 / sqrt(var + eps): the hardware's estimate and one Newton step, within 2
@@ -71,8 +72,9 @@ template <typename T, int V> NEON_DEV void load_clipped(nh_raw<T, V>& r, const T
     else if (n > 0) r.load_partial(p, n);
     else r.zero();
 }
-template <typename T, int V> NEON_DEV void store_clipped(const nh_out<T, V>& o, T* p, int n) {
-    if (n >= V) o.store(p);
+template <typename T, int V> NEON_DEV void store_clipped(const nh_out<T, V>& o, T* p, int n, bool stream = false) {
+    if (n >= V && stream) o.store_stream(p);
+    else if (n >= V) o.store(p);
     else if (n > 0) o.store_partial(p, n);
 }
 // V fp32 values at p, the ones behind n zero
@@ -86,44 +88,122 @@ template <int V> NEON_DEV void load_floats(float (&f)[V], const float* p, int n)
 }
 NEON_DEV int clip(long long left, int v) { return left >= v ? v : (left > 0 ? (int)left : 0); }
 
+// Threads TPR per row (64: a wave, four rows per workgroup at a time).
+template <int TPR> struct RowShape {
+    static constexpr int NT = TPR == 64 ? 256 : TPR, RPB = TPR == 64 ? 4 : 1;
+};
+
 // ---------------------------------------------------------------------------
-// rows, forward: TPR threads hold one row in registers (NV 16-byte vectors
-// each), so x is read once although the variance is taken around the mean.
+// rows, forward.  TPR threads hold one row in registers (NV 16-byte vectors
+// each), so x is read once although the variance is taken around the mean.  A
+// workgroup walks over rows with gamma and beta kept, and the next row is asked
+// for before this one is summed up: loads return in the order of issue, stores
+// among them, so a load behind this row's stores would wait for them.  The rows
+// take turns in two sets of registers; moving the next row into this one's place
+// would wait for it.
 // ---------------------------------------------------------------------------
-template <typename T, int TPR, int NV>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void ln_rows_fprop_kernel(LnArgs a) {
-    constexpr int V = vec<T>::V;
-    constexpr int RPB = TPR == 64 ? 4 : 1;
+template <typename T, int TPR, int NV> __global__ __launch_bounds__(RowShape<TPR>::NT) void ln_rows_fprop_kernel(LnArgs a) {
+    constexpr int V = vec<T>::V, RPB = RowShape<TPR>::RPB;
     __shared__ float2 slots[2][TPR / 64];
-    const size_t row = (size_t)blockIdx.x * RPB + threadIdx.x / TPR;
     const int t = threadIdx.x % TPR;
+    const float inv_f = 1.0f / (float)a.features;
+    const size_t step = (size_t)gridDim.x * RPB;
+    size_t row = (size_t)blockIdx.x * RPB + threadIdx.x / TPR;
     if (TPR == 64 && row >= a.positions) return;
+    int n[NV];
+    nh_raw<T, V> even[NV], odd[NV];
+    const auto load = [&](nh_raw<T, V> (&to)[NV], size_t at) {
+        const T* x = (const T*)a.x + at * a.ld_x;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) load_clipped(to[k], x + (uint32_t)(k * TPR + t) * V, n[k]);
+    };
+#pragma unroll
+    for (int k = 0; k < NV; ++k) n[k] = clip((long long)a.features - (uint32_t)(k * TPR + t) * V, V);
+    load(even, row);
+    float g[NV][V], b[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        load_floats<V>(g[k], a.gamma + (uint32_t)(k * TPR + t) * V, n[k]);
+        load_floats<V>(b[k], a.beta + (uint32_t)(k * TPR + t) * V, n[k]);
+    }
+    const auto normalise = [&](const nh_raw<T, V> (&r)[NV], size_t at) {
+        float s = 0.0f, unused = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += r[k].get(j);
+        row_sum2<TPR>(s, unused, slots[0]);
+        const float mu = s * inv_f;
+        float q = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = r[k].get(j) - mu;
+                q = __builtin_fmaf(d, j < n[k] ? d : 0.0f, q);
+            }
+        }
+        row_sum2<TPR>(q, unused, slots[1]);
+        const float var = q * inv_f;
+        const float rs = inv_std(var, a.eps);
+        T* y = (T*)a.out + at * a.ld_out;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            nh_out<T, V> o;
+            o.clear();
+#pragma unroll
+            for (int j = 0; j < V; ++j) o.set(j, __builtin_fmaf((r[k].get(j) - mu) * rs, g[k][j], b[k][j]));
+            store_clipped(o, y + (uint32_t)(k * TPR + t) * V, n[k], a.stream);
+        }
+        if (t == 0) {
+            a.mean[at] = mu;
+            a.var[at] = var;
+        }
+    };
+    for (;;) {
+        if (row + step < a.positions) load(odd, row + step);
+        normalise(even, row);
+        row += step;
+        if (row >= a.positions) return;
+        if (row + step < a.positions) load(even, row + step);
+        normalise(odd, row);
+        row += step;
+        if (row >= a.positions) return;
+    }
+}
+
+// Rows of more features than that leaves registers for: one workgroup per row,
+// gamma and beta read when they are needed.
+template <typename T, int NV> __global__ __launch_bounds__(1024) void ln_rows_fprop_wide_kernel(LnArgs a) {
+    constexpr int V = vec<T>::V, TPR = 1024;
+    __shared__ float2 slots[2][TPR / 64];
+    const size_t row = blockIdx.x;
+    const int t = threadIdx.x;
     const T* x = (const T*)a.x + row * a.ld_x;
     T* y = (T*)a.out + row * a.ld_out;
     const float inv_f = 1.0f / (float)a.features;
-
+    const auto left = [&](int k) { return clip((long long)a.features - (uint32_t)(k * TPR + t) * V, V); };
     nh_raw<T, V> r[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) load_clipped(r[k], x + (uint32_t)(k * TPR + t) * V, left(k));
     float s = 0.0f, unused = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const uint32_t c = (uint32_t)(k * TPR + t) * V;
-        load_clipped(r[k], x + c, clip((long long)a.features - c, V));
-    }
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int j = 0; j < V; ++j) s += r[k].get(j);
+        r[k].keep();
+    }
     row_sum2<TPR>(s, unused, slots[0]);
     const float mu = s * inv_f;
     float q = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int n = clip((long long)a.features - (uint32_t)(k * TPR + t) * V, V);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float d = r[k].get(j) - mu;
-            q = __builtin_fmaf(d, j < n ? d : 0.0f, q);
+            q = __builtin_fmaf(d, j < left(k) ? d : 0.0f, q);
         }
+        r[k].keep();
     }
     row_sum2<TPR>(q, unused, slots[1]);
     const float var = q * inv_f;
@@ -135,8 +215,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void ln_rows_fprop_kernel(Ln
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const uint32_t c = (uint32_t)(k * TPR + t) * V;
-        const int n = clip((long long)a.features - c, V);
-        if (n <= 0) continue;
+        const int n = left(k);
         float g[V], b[V];
         load_floats<V>(g, a.gamma + c, n);
         load_floats<V>(b, a.beta + c, n);
@@ -145,6 +224,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void ln_rows_fprop_kernel(Ln
 #pragma unroll
         for (int j = 0; j < V; ++j) o.set(j, __builtin_fmaf((r[k].get(j) - mu) * rs, g[j], b[j]));
         store_clipped(o, y + c, n);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -210,63 +290,89 @@ template <typename T> __global__ __launch_bounds__(1024) void ln_rows_fprop_long
 // each workgroup leaves one partial row of both (gridDim.x of them), which
 // ln_param_kernel adds up in a fixed order.
 // ---------------------------------------------------------------------------
-template <typename T, int TPR, int NV>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void ln_rows_bprop_kernel(LnArgs a) {
-    constexpr int V = vec<T>::V;
-    constexpr int RPB = TPR == 64 ? 4 : 1;
+template <typename T, int TPR, int NV> __global__ __launch_bounds__(RowShape<TPR>::NT) void ln_rows_bprop_kernel(LnArgs a) {
+    constexpr int V = vec<T>::V, RPB = RowShape<TPR>::RPB;
     __shared__ float2 slots[2][TPR / 64];
     const int t = threadIdx.x % TPR;
     const float inv_f = 1.0f / (float)a.features;
-    float g[NV][V], dg[NV][V], db[NV][V];
+    const size_t step = (size_t)gridDim.x * RPB;
+    size_t row = (size_t)blockIdx.x * RPB + threadIdx.x / TPR;
     int n[NV];
 #pragma unroll
+    for (int k = 0; k < NV; ++k) n[k] = clip((long long)a.features - (uint32_t)(k * TPR + t) * V, V);
+    struct Row {
+        nh_raw<T, V> x[NV], d[NV];
+        float mean, var;
+    };
+    Row even, odd;
+    const auto load = [&](Row& to, size_t at) {
+        to.mean = a.mean[at];
+        to.var = a.var[at];
+        const T* x = (const T*)a.x + at * a.ld_x;
+        const T* dy = (const T*)a.dy + at * a.ld_dy;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            load_clipped(to.x[k], x + (uint32_t)(k * TPR + t) * V, n[k]);
+            load_clipped(to.d[k], dy + (uint32_t)(k * TPR + t) * V, n[k]);
+        }
+    };
+    if (row < a.positions) load(even, row);
+    float g[NV][V], dg[NV][V], db[NV][V];
+#pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const uint32_t c = (uint32_t)(k * TPR + t) * V;
-        n[k] = clip((long long)a.features - c, V);
-        load_floats<V>(g[k], a.gamma + c, n[k]);
+        load_floats<V>(g[k], a.gamma + (uint32_t)(k * TPR + t) * V, n[k]);
 #pragma unroll
         for (int j = 0; j < V; ++j) dg[k][j] = db[k][j] = 0.0f;
     }
-    int parity = 0;
-    const size_t step = (size_t)gridDim.x * RPB;
-    for (size_t row = (size_t)blockIdx.x * RPB + threadIdx.x / TPR; row < a.positions; row += step) {
-        const T* x = (const T*)a.x + row * a.ld_x;
-        const T* dy = (const T*)a.dy + row * a.ld_dy;
-        T* dx = (T*)a.out + row * a.ld_out;
-        nh_raw<T, V> rx[NV], rd[NV];
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const uint32_t c = (uint32_t)(k * TPR + t) * V;
-            load_clipped(rx[k], x + c, n[k]);
-            load_clipped(rd[k], dy + c, n[k]);
-        }
-        const float mu = a.mean[row], rs = inv_std(a.var[row], a.eps);
+    const auto go = [&](Row& r, size_t at, float2* slot) {
+        const float mu = r.mean, rs = inv_std(r.var, a.eps);
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float h = (rx[k].get(j) - mu) * rs, d = rd[k].get(j), u = d * g[k][j];
+                const float h = (r.x[k].get(j) - mu) * rs, d = r.d[k].get(j), u = d * g[k][j];
                 s1 += u;
                 s2 = __builtin_fmaf(u, h, s2);
                 dg[k][j] = __builtin_fmaf(d, h, dg[k][j]);
                 db[k][j] += d;
             }
-        row_sum2<TPR>(s1, s2, slots[parity]);
-        parity ^= 1;
+            // (widened again below)
+            r.x[k].keep();
+            r.d[k].keep();
+        }
+        row_sum2<TPR>(s1, s2, slot);
         s1 *= inv_f;
         s2 *= inv_f;
+        T* dx = (T*)a.out + at * a.ld_out;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (n[k] <= 0) continue;
             nh_out<T, V> o;
             o.clear();
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float h = (rx[k].get(j) - mu) * rs, u = rd[k].get(j) * g[k][j];
+                const float h = (r.x[k].get(j) - mu) * rs, u = r.d[k].get(j) * g[k][j];
                 o.set(j, rs * ((u - s1) - h * s2));
             }
-            store_clipped(o, dx + (uint32_t)(k * TPR + t) * V, n[k]);
+            store_clipped(o, dx + (uint32_t)(k * TPR + t) * V, n[k], a.stream);
+        }
+    };
+    // two sets of registers in turn, see the forward kernel -- where they fit
+    if constexpr (TPR == 1024 && NV * V > 8) {
+        for (int turn = 0; row < a.positions; turn ^= 1) {
+            go(even, row, slots[turn]);
+            row += step;
+            if (row < a.positions) load(even, row);
+        }
+    } else {
+        while (row < a.positions) {
+            if (row + step < a.positions) load(odd, row + step);
+            go(even, row, slots[0]);
+            row += step;
+            if (row >= a.positions) break;
+            if (row + step < a.positions) load(even, row + step);
+            go(odd, row, slots[1]);
+            row += step;
         }
     }
     float* part = a.part + (size_t)blockIdx.x * 2 * a.features;
@@ -897,8 +1003,12 @@ template <typename T> __global__ __launch_bounds__(256) void ln_cols_bprop_finis
 // launch geometry
 // ---------------------------------------------------------------------------
 constexpr size_t LONG_ROW_FPROP = 65536;      // features one workgroup's registers hold
-constexpr size_t LONG_ROW_BPROP = 16384;
-constexpr unsigned ROW_GROUPS = 512;          // workgroups that walk the rows in the backward pass
+// features of a row that the backward kernel holds with its parameter sums (16 fp32 features
+// per thread of 1024 spill 61 registers)
+size_t long_row_bprop(int dtype) { return dtype == NH_T_F32 ? 8192 : 16384; }
+constexpr size_t FPROP_THREADS = 2048, BPROP_THREADS = 512;       // per CU, of workgroups that walk over rows
+constexpr size_t BPROP_ROWS = 3;              // rows at least that a workgroup leaves one partial row for
+constexpr size_t STREAM_BYTES = (size_t)256 << 20;           // what the last-level cache holds
 constexpr unsigned LONG_ROW_RUNS = 64;        // row runs per feature strip in ln_rows_params_kernel
 constexpr size_t COL_CHUNKS = 32;             // runs of tiles per strip of a split column kernel, at most
 
@@ -919,16 +1029,19 @@ ColSplit split_columns(const ColLimits& l, size_t features) {
     return {(uint32_t)(per * l.tile), (uint32_t)lm::ceil_div(tiles, per)};
 }
 
-unsigned row_groups(size_t features, size_t positions) {
-    const size_t per_block = features <= (size_t)64 * 16 ? 4 : 1;
-    const size_t blocks = lm::ceil_div(positions, per_block);
-    return (unsigned)(blocks < ROW_GROUPS ? blocks : ROW_GROUPS);
+// workgroups that walk over rows with `threads` each per row
+unsigned row_blocks(size_t positions, size_t threads, size_t per_cu) {
+    const size_t rows = threads == 64 ? 4 : 1, most = 256 * per_cu / (threads == 64 ? 256 : threads);
+    const size_t blocks = lm::ceil_div(positions, rows);
+    return (unsigned)(blocks < most ? blocks : most);
 }
+// threads per row of the backward kernel: at most 16 features each
+size_t bprop_threads(size_t features) { return features <= 64 * 16 ? 64 : features <= 256 * 16 ? 256 : 1024; }
 
 size_t partial_rows(size_t features, size_t positions, int dtype, bool columns) {
     if (columns) return strips_of(COL_BPROP, dtype, positions);
-    if (features > LONG_ROW_BPROP) return positions < LONG_ROW_RUNS ? positions : LONG_ROW_RUNS;
-    return row_groups(features, positions);
+    if (features > long_row_bprop(dtype)) return positions < LONG_ROW_RUNS ? positions : LONG_ROW_RUNS;
+    return row_blocks(lm::ceil_div(positions, BPROP_ROWS), bprop_threads(features), BPROP_THREADS);
 }
 
 size_t column_sum_bytes(const ColLimits& l, size_t features, size_t positions, int dtype) {
@@ -961,18 +1074,22 @@ template <typename T> int fprop_rows(const LnArgs& a, hipStream_t s) {
     constexpr size_t V = vec<T>::V;
     const size_t nvec = lm::ceil_div(a.features, V);
     if (a.positions > lm::MAX_BLOCKS) return lm::refuse("nh_ln_fprop", "too many positions for one launch");
-    const dim3 by4((unsigned)lm::ceil_div(a.positions, 4)), by1((unsigned)a.positions);
-#define LN_GO(TPR, NV) hipLaunchKernelGGL((ln_rows_fprop_kernel<T, TPR, NV>), TPR == 64 ? by4 : by1, dim3(TPR == 64 ? 256 : TPR), 0, s, a)
+    if (a.features > LONG_ROW_FPROP) {
+        hipLaunchKernelGGL((ln_rows_fprop_long_kernel<T>), dim3((unsigned)a.positions), dim3(1024), 0, s, a);
+        return lm::launched("nh_ln_fprop");
+    }
+#define LN_WIDE(NV) hipLaunchKernelGGL((ln_rows_fprop_wide_kernel<T, NV>), dim3((unsigned)a.positions), dim3(1024), 0, s, a)
+#define LN_GO(TPR, NV) hipLaunchKernelGGL((ln_rows_fprop_kernel<T, TPR, NV>), dim3(row_blocks(a.positions, TPR, FPROP_THREADS)), dim3(RowShape<TPR>::NT), 0, s, a)
     if (nvec <= 64) LN_GO(64, 1);
     else if (nvec <= 128) LN_GO(64, 2);
     else if (nvec <= 256) LN_GO(256, 1);
     else if (nvec <= 512) LN_GO(256, 2);
-    else if (nvec <= 1024) LN_GO(256, 4);
+    else if (nvec <= 1024) LN_GO(512, 2);
     else if (nvec <= 2048) LN_GO(1024, 2);
-    else if (nvec <= 4096) LN_GO(1024, 4);
-    else if (nvec <= 8192) LN_GO(1024, 8);
-    else if (a.features > LONG_ROW_FPROP) hipLaunchKernelGGL((ln_rows_fprop_long_kernel<T>), by1, dim3(1024), 0, s, a);
-    else if constexpr (sizeof(T) == 4) LN_GO(1024, 16);
+    else if (nvec <= 4096) LN_WIDE(4);
+    else if (nvec <= 8192) LN_WIDE(8);
+    else if constexpr (sizeof(T) == 4) LN_WIDE(16);
+#undef LN_WIDE
 #undef LN_GO
     return lm::launched("nh_ln_fprop");
 }
@@ -1009,7 +1126,7 @@ template <typename T> int bprop_rows(const LnArgs& a, hipStream_t s) {
     constexpr size_t V = vec<T>::V;
     const size_t nvec = lm::ceil_div(a.features, V);
     const size_t rows = partial_rows(a.features, a.positions, code_of<T>(), false);
-    if (a.features > LONG_ROW_BPROP) {
+    if (a.features > long_row_bprop(code_of<T>())) {
         if (a.positions > lm::MAX_BLOCKS) return lm::refuse("nh_ln_bprop", "too many positions for one launch");
         const size_t per = lm::ceil_div(a.positions, rows);
         // (the sums first: dx may take the place of dy)
@@ -1019,14 +1136,14 @@ template <typename T> int bprop_rows(const LnArgs& a, hipStream_t s) {
         return lm::launched("nh_ln_bprop");
     }
     const dim3 grid((unsigned)rows);
-#define LN_GO(TPR, NV) hipLaunchKernelGGL((ln_rows_bprop_kernel<T, TPR, NV>), grid, dim3(TPR == 64 ? 256 : TPR), 0, s, a)
+#define LN_GO(TPR, NV) hipLaunchKernelGGL((ln_rows_bprop_kernel<T, TPR, NV>), grid, dim3(RowShape<TPR>::NT), 0, s, a)
     if (a.features <= 64 * V) LN_GO(64, 1);
     else if (a.features <= 64 * 8) LN_GO(64, 8 / V < 2 ? 1 : 2);
     else if (a.features <= 64 * 16) LN_GO(64, 16 / V);
     else if (a.features <= 256 * 8) LN_GO(256, 8 / V);
     else if (a.features <= 256 * 16) LN_GO(256, 16 / V);
     else if (a.features <= 1024 * 8) LN_GO(1024, 8 / V);
-    else LN_GO(1024, 16 / V);
+    else if constexpr (sizeof(T) == 2) LN_GO(1024, 16 / V);
 #undef LN_GO
     add_params(a, rows, s);
     return lm::launched("nh_ln_bprop");
@@ -1077,6 +1194,7 @@ int nh_ln_fprop(void* y, float* mean, float* var, const void* x, const float* ga
     LnArgs a = {};
     a.x = x; a.out = y; a.gamma = gamma; a.beta = beta; a.mean = mean; a.var = var; a.part = (float*)workspace;
     a.eps = eps; a.features = (uint32_t)features; a.positions = positions; a.ld_x = ld_x; a.ld_out = ld_y;
+    a.stream = 2 * features * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
     return lm::by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         return axis == 1 ? fprop_rows<T>(a, (hipStream_t)stream) : fprop_cols<T>(a, (hipStream_t)stream);
@@ -1098,6 +1216,7 @@ int nh_ln_bprop(void* dx, float* dgamma, float* dbeta, const void* dy, const voi
     a.x = x; a.dy = dy; a.out = dx; a.gamma = gamma; a.mean = const_cast<float*>(mean); a.var = const_cast<float*>(var);
     a.part = (float*)workspace; a.grads[0] = dgamma; a.grads[1] = dbeta;
     a.eps = eps; a.features = (uint32_t)features; a.positions = positions; a.ld_x = ld_x; a.ld_dy = ld_dy; a.ld_out = ld_dx;
+    a.stream = 3 * features * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
     if (positions == 0) {          // sums over no positions
         add_params(a, 0, (hipStream_t)stream);
         return lm::launched("nh_ln_bprop");

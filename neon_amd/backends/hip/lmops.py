@@ -16,6 +16,7 @@ a lookup table's gradient (:2591-2660) and cross-entropy
 follow those.
 """
 import math
+import operator
 
 import numpy as np
 
@@ -64,6 +65,9 @@ def _leading(t, axis, layout):
     return step_p if step_p >= features else None
 
 
+_address = operator.itemgetter(0)
+
+
 def _dense(t, axis):
     """a vector along ``axis`` without gaps"""
     return not t.take_array and (t.shape[axis] == 1 or t.strides[axis] == 1)
@@ -99,6 +103,42 @@ def _interleaved(a, b):
 
 class LanguageModelOps(object):
     """see the module's docstring"""
+
+    # -- calls seen before --------------------------------------------------------------
+    # A call whose tensors have the shapes, strides and types of an earlier one needs none of that
+    # looked at again: ``_lm_forms`` keeps, by these and by nothing else, the constant arguments of
+    # the library call.  What depends on addresses (overlap) and on attributes a program may change
+    # (rounding) is looked at every time.
+    def _lm_form(self, name, axis, tensors, outputs):
+        """(key, constant arguments or None) of a call whose first ``outputs``
+        tensors are written"""
+        try:
+            key = (name, axis) + tuple([t._geom[1:] for t in tensors])
+            tail = self._lm_forms.get(key)
+        except (AttributeError, TypeError):
+            return None, None
+        if tail is None:
+            return key, None
+        for t in tensors[:outputs]:
+            if t.rounding:
+                return key, None
+        # (every tensor of a kept form is read and written in place; where two might share memory the
+        # long way decides)
+        spans = sorted([(t.gpudata, t) for t in tensors], key=_address)
+        end = 0
+        for at, t in spans:
+            if at < end:
+                return key, None
+            end = at + (t.nbytes if t.is_contiguous else self._lm_byte_span(t)[1] - at)
+        if self._deferred or self._pending:
+            self._flush()
+        return key, tail
+
+    def _lm_keep(self, key, temps, tail):
+        if key is not None and not temps:
+            if len(self._lm_forms) >= 4096:         # a program of ever new shapes
+                self._lm_forms.clear()
+            self._lm_forms[key] = tail
 
     # -- arguments ----------------------------------------------------------------------
     def _lm_tensors(self, axis, outputs, inputs, aliases=()):
@@ -223,6 +263,12 @@ class LanguageModelOps(object):
         1), xmean and xvar (1, positions); with ``axis=1`` all of them
         transposed.  x and y are float32, float16 or bfloat16 alike, the rest is
         float32.  y may be x."""
+        key, tail = self._lm_form("ln", axis, (y, xmean, xvar, x, gamma, beta), 3)
+        if tail is not None:
+            ws, ws_bytes = self._lm_workspace(tail[6])
+            hiprt.check(self.rt.lib.nh_ln_fprop(y.gpudata, xmean.gpudata, xvar.gpudata, x.gpudata, gamma.gpudata,
+                                                beta.gpudata, eps, *tail[:6], ws, ws_bytes, self.rt.stream))
+            return
         self._lm_tensors(axis, (y, xmean, xvar), (x, gamma, beta), ((y, x),))
         code = _storage("x", x)
         features, positions = x.shape[axis], x.shape[1 - axis]
@@ -245,10 +291,12 @@ class LanguageModelOps(object):
             gamma, beta = self._lm_vector_in(gamma, axis, temps), self._lm_vector_in(beta, axis, temps)
             mean, var = (self._lm_vector_out(t, 1 - axis, temps, back) for t in (xmean, xvar))
             rt = self.rt
-            ws, ws_bytes = self._lm_workspace(rt.lib.nh_ln_workspace_bytes(0, code, layout, features, positions))
+            need = rt.lib.nh_ln_workspace_bytes(0, code, layout, features, positions)
+            ws, ws_bytes = self._lm_workspace(need)
+            tail = (code, layout, features, positions, ld_x, ld_y)
             hiprt.check(rt.lib.nh_ln_fprop(out.gpudata, mean.gpudata, var.gpudata, xin.gpudata, gamma.gpudata,
-                                           beta.gpudata, eps, code, layout, features, positions, ld_x, ld_y,
-                                           ws, ws_bytes, rt.stream))
+                                           beta.gpudata, eps, *tail, ws, ws_bytes, rt.stream))
+            self._lm_keep(key, temps, tail + (need,))
             self._lm_copy_back(back)
         finally:
             self._lm_release(temps)
@@ -259,6 +307,13 @@ class LanguageModelOps(object):
         ``delta_in`` with respect to y and the saved statistics.  Shapes and
         types as there; sums over positions are taken in a fixed order.
         delta_out may be delta_in or x."""
+        key, tail = self._lm_form("ln grad", axis, (delta_out, grad_gamma, grad_beta, delta_in, x, xmean, xvar, gamma), 3)
+        if tail is not None:
+            ws, ws_bytes = self._lm_workspace(tail[7])
+            hiprt.check(self.rt.lib.nh_ln_bprop(delta_out.gpudata, grad_gamma.gpudata, grad_beta.gpudata, delta_in.gpudata,
+                                                x.gpudata, xmean.gpudata, xvar.gpudata, gamma.gpudata, eps, *tail[:7],
+                                                ws, ws_bytes, self.rt.stream))
+            return
         self._lm_tensors(axis, (delta_out, grad_gamma, grad_beta), (delta_in, x, xmean, xvar, gamma),
                          ((delta_out, delta_in), (delta_out, x)))
         code = _storage("x", x)
@@ -283,10 +338,12 @@ class LanguageModelOps(object):
             mean, var = (self._lm_vector_in(t, 1 - axis, temps) for t in (xmean, xvar))
             dgamma, dbeta = (self._lm_vector_out(t, axis, temps, back) for t in (grad_gamma, grad_beta))
             rt = self.rt
-            ws, ws_bytes = self._lm_workspace(rt.lib.nh_ln_workspace_bytes(1, code, layout, features, positions))
+            need = rt.lib.nh_ln_workspace_bytes(1, code, layout, features, positions)
+            ws, ws_bytes = self._lm_workspace(need)
+            tail = (code, layout, features, positions, ld_x, ld_dy, ld_dx)
             hiprt.check(rt.lib.nh_ln_bprop(dx.gpudata, dgamma.gpudata, dbeta.gpudata, dy.gpudata, xin.gpudata,
-                                           mean.gpudata, var.gpudata, gamma.gpudata, eps, code, layout, features,
-                                           positions, ld_x, ld_dy, ld_dx, ws, ws_bytes, rt.stream))
+                                           mean.gpudata, var.gpudata, gamma.gpudata, eps, *tail, ws, ws_bytes, rt.stream))
+            self._lm_keep(key, temps, tail + (need,))
             self._lm_copy_back(back)
         finally:
             self._lm_release(temps)
@@ -310,6 +367,12 @@ class LanguageModelOps(object):
         W.  inputs holds int32 ids, in row-major order whatever its shape; W is
         (vocabulary, embedding size); outputs (embedding size, positions) for
         ``axis=0``, (positions, embedding size) for ``axis=1``."""
+        pad = -1 if pad_idx is None else int(pad_idx)
+        key, tail = self._lm_form("lut", axis, (outputs, inputs, W), 1)
+        if tail is not None:
+            hiprt.check(self.rt.lib.nh_embed_fprop(outputs.gpudata, W.gpudata, inputs.gpudata, scale, *tail, pad,
+                                                   self.rt.stream))
+            return
         self._lm_tensors(axis, (outputs,), (inputs, W))
         code = _storage("W", W)
         vocab, embed = W.shape
@@ -327,8 +390,9 @@ class LanguageModelOps(object):
             layout = self._lm_layout(axis, (outputs,))
             out, ld_out = self._lm_out(outputs, axis, layout, temps, back)
             rt = self.rt
-            hiprt.check(rt.lib.nh_embed_fprop(out.gpudata, table.gpudata, ids.gpudata, scale, code, layout, count, embed,
-                                              vocab, ld_w, ld_out, -1 if pad_idx is None else int(pad_idx), rt.stream))
+            tail = (code, layout, count, embed, vocab, ld_w, ld_out)
+            hiprt.check(rt.lib.nh_embed_fprop(out.gpudata, table.gpudata, ids.gpudata, scale, *tail, pad, rt.stream))
+            self._lm_keep(key, temps, tail)
             self._lm_copy_back(back)
         finally:
             self._lm_release(temps)
@@ -340,6 +404,13 @@ class LanguageModelOps(object):
         do not occur.  ``beta=0`` defines every row of dW, ``beta=1`` adds to it.
         error has the shape outputs had; sums are taken in a fixed order, in
         float32."""
+        pad = -1 if pad_idx is None else int(pad_idx)
+        key, tail = self._lm_form("lut grad", axis, (dW, inputs, error), 1)
+        if tail is not None:
+            ws, ws_bytes = self._lm_workspace(tail[7])
+            hiprt.check(self.rt.lib.nh_embed_update(dW.gpudata, error.gpudata, inputs.gpudata, scale, beta, *tail[:7], pad,
+                                                    ws, ws_bytes, self.rt.stream))
+            return
         self._lm_tensors(axis, (dW,), (inputs, error))
         code = _storage("dW", dW)
         vocab, embed = dW.shape
@@ -355,10 +426,12 @@ class LanguageModelOps(object):
             layout = self._lm_layout(axis, (error,))
             err, ld_err = self._lm_in(error, axis, layout, temps)
             rt = self.rt
-            ws, ws_bytes = self._lm_workspace(rt.lib.nh_embed_update_workspace_bytes(code, layout, count, embed, vocab))
-            hiprt.check(rt.lib.nh_embed_update(table.gpudata, err.gpudata, ids.gpudata, scale, beta, code, layout, count,
-                                               embed, vocab, ld_dw, ld_err, -1 if pad_idx is None else int(pad_idx),
+            need = rt.lib.nh_embed_update_workspace_bytes(code, layout, count, embed, vocab)
+            ws, ws_bytes = self._lm_workspace(need)
+            tail = (code, layout, count, embed, vocab, ld_dw, ld_err)
+            hiprt.check(rt.lib.nh_embed_update(table.gpudata, err.gpudata, ids.gpudata, scale, beta, *tail, pad,
                                                ws, ws_bytes, rt.stream))
+            self._lm_keep(key, temps, tail + (need,))
             self._lm_copy_back(back)
         finally:
             self._lm_release(temps)
@@ -400,6 +473,13 @@ class LanguageModelOps(object):
         positions), loss (1, positions), stats (4, positions); with ``axis=1``
         all of them transposed.  y and t are float32, float16 or bfloat16, loss
         and stats float32; at most 1024 entries."""
+        key, tail = self._lm_form("distill", axis, (loss, stats, y, ids, t), 2)
+        if tail is not None:
+            ws, ws_bytes = self._lm_workspace(tail[8])
+            hiprt.check(self.rt.lib.nh_distill_fprop(loss.gpudata, stats.gpudata, y.gpudata, ids.gpudata, t.gpudata,
+                                                     self._lm_temperature(temperature), *tail[:8], ws, ws_bytes,
+                                                     self.rt.stream))
+            return
         self._lm_tensors(axis, (loss, stats), (y, ids, t))
         code, t_code = _storage("y", y), _storage("t", t)
         temperature = self._lm_temperature(temperature)
@@ -416,11 +496,14 @@ class LanguageModelOps(object):
             if t.take_array:
                 t, _ = self._lm_in(t, axis, layout, temps)
             rt, vocab = self.rt, y.shape[axis]
-            ws, ws_bytes = self._lm_workspace(rt.lib.nh_distill_workspace_bytes(0, code, layout, vocab, positions, entries))
+            need = rt.lib.nh_distill_workspace_bytes(0, code, layout, vocab, positions, entries)
+            ws, ws_bytes = self._lm_workspace(need)
             strides = hiprt.int64s(ids.strides[axis], ids.strides[1 - axis], t.strides[axis], t.strides[1 - axis],
                                    loss.strides[1 - axis], stats.strides[axis], stats.strides[1 - axis])
-            hiprt.check(rt.lib.nh_distill_fprop(loss.gpudata, stats.gpudata, z.gpudata, ids.gpudata, t.gpudata, temperature, code, t_code, layout, vocab,
-                                                positions, entries, ld_z, strides, ws, ws_bytes, rt.stream))
+            tail = (code, t_code, layout, vocab, positions, entries, ld_z, strides)
+            hiprt.check(rt.lib.nh_distill_fprop(loss.gpudata, stats.gpudata, z.gpudata, ids.gpudata, t.gpudata, temperature,
+                                                *tail, ws, ws_bytes, rt.stream))
+            self._lm_keep(key, temps, tail + (need,))
         finally:
             self._lm_release(temps)
 
@@ -434,6 +517,16 @@ class LanguageModelOps(object):
         and 0 at positions without entries.  delta is shaped and typed like y
         and must not share its memory; stats is what the forward pass left."""
         tensor_weight = isinstance(weight, self._lm_tensor_base)
+        key, tail = self._lm_form("distill grad" if tensor_weight else "distill grad, one weight", axis,
+                                  (delta, y, ids, t, stats) + ((weight,) if tensor_weight else ()), 1)
+        if tail is not None:
+            ws, ws_bytes = self._lm_workspace(tail[9])
+            hiprt.check(self.rt.lib.nh_distill_bprop(delta.gpudata, y.gpudata, ids.gpudata, t.gpudata, stats.gpudata,
+                                                     weight.gpudata if tensor_weight else None,
+                                                     1.0 if tensor_weight else float(weight),
+                                                     self._lm_temperature(temperature), *tail[:9], ws, ws_bytes,
+                                                     self.rt.stream))
+            return
         self._lm_tensors(axis, (delta,), (y, ids, t, stats) + ((weight,) if tensor_weight else ()))
         code, t_code = _storage("y", y), _storage("t", t)
         temperature = self._lm_temperature(temperature)
@@ -457,13 +550,16 @@ class LanguageModelOps(object):
             if tensor_weight and weight.take_array:
                 weight = self._lm_vector_in(weight, 1 - axis, temps)
             rt, vocab = self.rt, y.shape[axis]
-            ws, ws_bytes = self._lm_workspace(rt.lib.nh_distill_workspace_bytes(1, code, layout, vocab, positions, entries))
+            need = rt.lib.nh_distill_workspace_bytes(1, code, layout, vocab, positions, entries)
+            ws, ws_bytes = self._lm_workspace(need)
             strides = hiprt.int64s(ids.strides[axis], ids.strides[1 - axis], t.strides[axis], t.strides[1 - axis],
                                    stats.strides[axis], stats.strides[1 - axis], weight.strides[1 - axis] if tensor_weight else 0)
+            tail = (code, t_code, layout, vocab, positions, entries, ld_z, ld_dz, strides)
             hiprt.check(rt.lib.nh_distill_bprop(dz.gpudata, z.gpudata, ids.gpudata, t.gpudata, stats.gpudata,
                                                 weight.gpudata if tensor_weight else None,
-                                                1.0 if tensor_weight else float(weight), temperature, code, t_code, layout,
-                                                vocab, positions, entries, ld_z, ld_dz, strides, ws, ws_bytes, rt.stream))
+                                                1.0 if tensor_weight else float(weight), temperature, *tail, ws, ws_bytes,
+                                                rt.stream))
+            self._lm_keep(key, temps, tail + (need,))
             self._lm_copy_back(back)
         finally:
             self._lm_release(temps)

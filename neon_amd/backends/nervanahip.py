@@ -616,6 +616,7 @@ class NervanaHIPBase(object):
         self._rec_foreign = False     # the group being recorded made a call that is not a kernel launch
         self._lut_ws = None           # (pointer, bytes) scratch of compound_bprop_lut
         self._lm_ws = None            # (pointer, bytes) scratch of the language-model operators
+        self._lm_forms = {}           # shapes, strides and types of their calls -> constant arguments
         self._originals = frozenset() # ids of handles whose reads mean "before the running group" (compensated_sum)
         self._rec_single = None
         self._temp_pool = {}

@@ -44,6 +44,7 @@ struct DistillArgs {
     nh_pair* part;          // forward: (maximum, sum) per position and chunk
     uint2* target;          // backward, columns: (word, probability) per entry and position
     uint32_t chunk, chunks;
+    bool stream;            // the logits are more than the last-level cache holds: read and written past it
 };
 
 NEON_DEV float load_t(const DistillArgs& a, uint32_t k, size_t n) {
@@ -102,9 +103,51 @@ NEON_DEV Lse lse_wave(Lse v, float c) {
 NEON_DEV float wave_sum(float v) { return nh_wave_allreduce<nh_op_sum, 64>(v); }
 NEON_DEV float wave_max(float v) { return nh_wave_allreduce<nh_op_max, 64>(v); }
 
+// One wave, with the student's state of position n: the teacher's entries, the
+// loss and the statistics.  z[v * step] is the logit of word v.
+template <typename T> NEON_DEV void finish_position(const DistillArgs& a, size_t n, Lse st, const T* z, size_t step) {
+    const int lane = threadIdx.x & 63;
+    const float log_s = logf(st.s);
+    float top = -NH_INF;
+    for (uint32_t k = lane; k < a.entries; k += 64)
+        if (is_word(load_id(a, k, n), a.vocab)) top = nh_max(top, load_t(a, k, n));
+    top = wave_max(top);
+    const bool some = top != -NH_INF;
+    const float top0 = some ? top : 0.0f;
+    float sum = 0.0f;
+    for (uint32_t k = lane; k < a.entries; k += 64)
+        if (is_word(load_id(a, k, n), a.vocab)) sum += expf((load_t(a, k, n) - top0) * a.inv_t);
+    sum = wave_sum(sum);
+    const float log_t = logf(sum);
+    float loss = 0.0f;
+    for (uint32_t k = lane; k < a.entries && some; k += 64) {
+        const int id = load_id(a, k, n);
+        if (!is_word(id, a.vocab)) continue;
+        const float log_p = (load_t(a, k, n) - top0) * a.inv_t - log_t;
+        const float p = expf(log_p);
+        const float log_q = ((float)z[(size_t)id * step] - st.m) * a.inv_t - log_s;
+        if (p != 0.0f) loss = __builtin_fmaf(p, log_p - log_q, loss);
+    }
+    loss = wave_sum(loss);
+    if (lane == 0) {
+        a.loss[(long long)n * a.loss_n] = a.temperature * a.temperature * loss;
+        float* p = a.stats + (long long)n * a.stat_n;
+        p[0] = st.m;
+        p[a.stat_k] = log_s;
+        p[2 * a.stat_k] = top;
+        p[3 * a.stat_k] = log_t;
+    }
+}
+
+template <typename T, int V> NEON_DEV void load_logits(nh_raw<T, V>& r, const T* p, bool stream) {
+    if (stream) r.load_stream(p);
+    else r.load(p);
+}
+
 // ---------------------------------------------------------------------------
-// forward: (maximum, sum) of chunks of the vocabulary, then one wave per
-// position joins them in order and adds up the teacher's entries
+// forward: (maximum, sum) of chunks of the vocabulary.  A position whose
+// vocabulary is one chunk is finished by the same workgroup; otherwise one wave
+// per position joins the chunks in order.
 // ---------------------------------------------------------------------------
 template <typename T> __global__ __launch_bounds__(256) void distill_rows_lse_kernel(DistillArgs a) {
     constexpr int V = vec<T>::V, AHEAD = 4;
@@ -115,18 +158,34 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_lse_ke
     const T* z = (const T*)a.z + n * a.ld_z;
     const float c = a.inv_t * LOG2E;
     Lse st = {-NH_INF, 0.0f};
+    // batches of AHEAD vectors per thread, the next one on its way while one is added up
+    constexpr uint32_t BATCH = AHEAD * 256 * V;
+    const uint32_t batches = (i1 - i0) / BATCH;
     uint32_t i = i0 + threadIdx.x * V;
-    for (; i + (AHEAD - 1) * 256 * V + V <= i1; i += AHEAD * 256 * V) {
-        nh_raw<T, V> r[AHEAD];
+    nh_raw<T, V> even[AHEAD], odd[AHEAD];
+    const auto load = [&](nh_raw<T, V> (&r)[AHEAD], uint32_t at) {
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) r[k].load(z + i + k * 256 * V);
+        for (int k = 0; k < AHEAD; ++k) load_logits(r[k], z + at + k * 256 * V, a.stream);
+    };
+    const auto add = [&](const nh_raw<T, V> (&r)[AHEAD]) {
         float x[AHEAD * V];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
 #pragma unroll
             for (int j = 0; j < V; ++j) x[k * V + j] = r[k].get(j);
         lse_add<AHEAD * V>(st, x, c);
+    };
+    if (batches) load(even, i);
+    for (uint32_t b = 0; b < batches; b += 2) {
+        if (b + 1 < batches) load(odd, i + BATCH);
+        add(even);
+        if (b + 1 < batches) {
+            if (b + 2 < batches) load(even, i + 2 * BATCH);
+            add(odd);
+        }
+        i += 2 * BATCH;
     }
+    i = i0 + batches * BATCH + threadIdx.x * V;
     for (; i < i1; i += 256 * V) {
         nh_raw<T, V> r;
         const int left = i1 - i < V ? (int)(i1 - i) : V;
@@ -140,12 +199,16 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_lse_ke
     st = lse_wave(st, c);
     if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = st;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < 64) {
         st = lse_join(lse_join(slots[0], slots[1], c), lse_join(slots[2], slots[3], c), c);
+        if (a.chunks == 1) {
+            finish_position(a, n, st, z, 1);
+            return;
+        }
         nh_pair p;
         p.v = st.m;
         p.i = __builtin_bit_cast(int, st.s);
-        a.part[(size_t)blockIdx.x] = p;      // [n][chunk]
+        if (threadIdx.x == 0) a.part[(size_t)blockIdx.x] = p;      // [n][chunk]
     }
 }
 
@@ -206,49 +269,17 @@ template <typename T> __global__ __launch_bounds__(256) void distill_cols_lse_ke
     }
 }
 
+// positions whose vocabulary was split, and the columns layout: a wave per position
 template <typename T> __global__ __launch_bounds__(256) void distill_finish_kernel(DistillArgs a, size_t z_n, size_t z_v) {
     const size_t n = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
     if (n >= a.positions) return;
     const float c = a.inv_t * LOG2E;
     Lse st = {-NH_INF, 0.0f};
-    for (uint32_t i = lane; i < a.chunks; i += 64) {
+    for (uint32_t i = threadIdx.x & 63; i < a.chunks; i += 64) {
         const nh_pair p = a.part[n * a.chunks + i];
         st = lse_join(st, {p.v, __builtin_bit_cast(float, p.i)}, c);
     }
-    st = lse_wave(st, c);
-    const float log_s = logf(st.s);
-
-    float top = -NH_INF;
-    for (uint32_t k = lane; k < a.entries; k += 64)
-        if (is_word(load_id(a, k, n), a.vocab)) top = nh_max(top, load_t(a, k, n));
-    top = wave_max(top);
-    const bool some = top != -NH_INF;
-    const float top0 = some ? top : 0.0f;
-    float sum = 0.0f;
-    for (uint32_t k = lane; k < a.entries; k += 64)
-        if (is_word(load_id(a, k, n), a.vocab)) sum += expf((load_t(a, k, n) - top0) * a.inv_t);
-    sum = wave_sum(sum);
-    const float log_t = logf(sum);
-    float loss = 0.0f;
-    const T* z = (const T*)a.z + n * z_n;
-    for (uint32_t k = lane; k < a.entries && some; k += 64) {
-        const int id = load_id(a, k, n);
-        if (!is_word(id, a.vocab)) continue;
-        const float log_p = (load_t(a, k, n) - top0) * a.inv_t - log_t;
-        const float p = expf(log_p);
-        const float log_q = ((float)z[(size_t)id * z_v] - st.m) * a.inv_t - log_s;
-        if (p != 0.0f) loss = __builtin_fmaf(p, log_p - log_q, loss);
-    }
-    loss = wave_sum(loss);
-    if (lane == 0) {
-        a.loss[(long long)n * a.loss_n] = a.temperature * a.temperature * loss;
-        float* p = a.stats + (long long)n * a.stat_n;
-        p[0] = st.m;
-        p[a.stat_k] = log_s;
-        p[2 * a.stat_k] = top;
-        p[3 * a.stat_k] = log_t;
-    }
+    finish_position(a, n, lse_wave(st, c), (const T*)a.z + n * z_n, z_v);
 }
 
 // ---------------------------------------------------------------------------
@@ -280,20 +311,38 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_bprop_
         ps[k] = entry_p(a, load_t(a, k, n), st);
     }
     const auto grad = [&](float x) { return some ? w * prob_q(x, a.inv_t, st.top, st.log_sum) : 0.0f; };
+    // batches of AHEAD vectors per thread.  Loads return in the order of issue, stores among them: the
+    // next batch is asked for before this one is stored.
+    constexpr uint32_t BATCH = AHEAD * 256 * V;
+    const uint32_t batches = (i1 - i0) / BATCH;
     uint32_t i = i0 + threadIdx.x * V;
-    for (; i + (AHEAD - 1) * 256 * V + V <= i1; i += AHEAD * 256 * V) {
-        nh_raw<T, V> r[AHEAD];
+    nh_raw<T, V> even[AHEAD], odd[AHEAD];
+    const auto load = [&](nh_raw<T, V> (&r)[AHEAD], uint32_t at) {
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) r[k].load(z + i + k * 256 * V);
+        for (int k = 0; k < AHEAD; ++k) load_logits(r[k], z + at + k * 256 * V, a.stream);
+    };
+    const auto put = [&](const nh_raw<T, V> (&r)[AHEAD], uint32_t at) {
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             nh_out<T, V> o;
             o.clear();
 #pragma unroll
             for (int j = 0; j < V; ++j) o.set(j, grad(r[k].get(j)));
-            o.store(dz + i + k * 256 * V);
+            if (a.stream) o.store_stream(dz + at + k * 256 * V);
+            else o.store(dz + at + k * 256 * V);
         }
+    };
+    if (batches) load(even, i);
+    for (uint32_t b = 0; b < batches; b += 2) {
+        if (b + 1 < batches) load(odd, i + BATCH);
+        put(even, i);
+        if (b + 1 < batches) {
+            if (b + 2 < batches) load(even, i + 2 * BATCH);
+            put(odd, i + BATCH);
+        }
+        i += 2 * BATCH;
     }
+    i = i0 + batches * BATCH + threadIdx.x * V;
     for (; i < i1; i += 256 * V) {
         nh_raw<T, V> r;
         const int left = i1 - i < V ? (int)(i1 - i) : V;
@@ -419,6 +468,8 @@ template <typename T> __global__ __launch_bounds__(256) void distill_cols_bprop_
 // launch geometry: enough workgroups to fill the device, each with enough of
 // the vocabulary to pay for its share of the teacher's entries
 // ---------------------------------------------------------------------------
+constexpr size_t STREAM_BYTES = (size_t)256 << 20;      // what the last-level cache holds
+
 struct Chunks {
     uint32_t len, count;
 };
@@ -489,6 +540,7 @@ int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* id
     a.ids_k = strides[0]; a.ids_n = strides[1]; a.t_k = strides[2]; a.t_n = strides[3]; a.loss_n = strides[4];
     a.stat_k = strides[5]; a.stat_n = strides[6];
     a.part = (nh_pair*)workspace; a.chunk = c.len; a.chunks = c.count;
+    a.stream = vocab * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
     return lm::by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const hipStream_t s = (hipStream_t)stream;
@@ -496,7 +548,8 @@ int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* id
         if (blocks > lm::MAX_BLOCKS || positions > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
         if (axis == 1) hipLaunchKernelGGL((distill_rows_lse_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
         else hipLaunchKernelGGL((distill_cols_lse_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-        hipLaunchKernelGGL((distill_finish_kernel<T>), dim3((unsigned)lm::ceil_div(positions, 4)), dim3(256), 0, s, a,
+        if (axis == 0 || c.count > 1)
+            hipLaunchKernelGGL((distill_finish_kernel<T>), dim3((unsigned)lm::ceil_div(positions, 4)), dim3(256), 0, s, a,
                            axis == 1 ? ld_z : (size_t)1, axis == 1 ? (size_t)1 : ld_z);
         return lm::launched(who);
     });
@@ -524,6 +577,7 @@ int nh_distill_bprop(void* dz, const void* z, const int32_t* ids, const void* t,
     a.ids_k = strides[0]; a.ids_n = strides[1]; a.t_k = strides[2]; a.t_n = strides[3]; a.stat_k = strides[4];
     a.stat_n = strides[5]; a.weight_n = strides[6];
     a.target = (uint2*)workspace; a.chunk = c.len; a.chunks = c.count;
+    a.stream = 2 * vocab * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
     return lm::by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const hipStream_t s = (hipStream_t)stream;

@@ -32,6 +32,7 @@ def be():
     b = object.__new__(NervanaHIP)
     b.rt = NoDevice()
     b._lm_ws, b._temp_pool, b._rec_temps = None, {}, None
+    b._lm_forms, b._pending, b._deferred = {}, [], []
     b._flush = lambda: None
     return b
 
@@ -203,6 +204,40 @@ def test_distillation_refusals(be):
     assert not be.rt.calls
 
 
+def test_a_call_of_a_form_seen_before_is_checked_where_it_can_differ(be):
+    """the second call of equal shapes takes the short way: same library call,
+    but overlap, rounding and changed layouts are still found"""
+    for axis in (0, 1):
+        be.rt.calls = []
+        a, b = ln_args(be, axis), ln_args(be, axis)
+        be.compound_fprop_ln(**a)
+        be.compound_fprop_ln(**b)
+        first, second = [c[1] for c in be.rt.calls if c[0] == "nh_ln_fprop"]
+        assert first[6:13] == second[6:13] and second[0] == b["y"].gpudata and second[3] == b["x"].gpudata
+        for bad in (dict(y=T(be, b["x"].shape, at=b["x"].gpudata + 4)), dict(xmean=T(be, b["xmean"].shape, at=b["x"].gpudata)),
+                    dict(xvar=b["xmean"]), dict(gamma=b["y"])):
+            with pytest.raises(ValueError):
+                be.compound_fprop_ln(**dict(b, **bad))
+        be.compound_fprop_ln(**dict(b, y=b["x"]))
+        be.compound_fprop_ln(**dict(b, beta=b["gamma"]))                  # inputs may share memory
+        b["y"].rounding = 10
+        with pytest.raises(NotImplementedError):
+            be.compound_fprop_ln(**b)
+        b["y"].rounding = 0
+        turned = dict(b, x=T(be, b["x"].shape[::-1]).T, y=T(be, b["x"].shape[::-1]).T)
+        be.compound_fprop_ln(**turned)
+        assert be.rt.calls[-1][1][8] == 1 - axis
+        with pytest.raises(TypeError):
+            be.compound_fprop_ln(**dict(b, x=T(be, b["x"].shape, np.float16)))
+        with pytest.raises(ValueError):
+            be.compound_fprop_ln(**dict(b, axis=1 - axis))
+    d = distill_args(be)
+    for _ in range(2):
+        be.compound_fprop_distill(**d)
+        with pytest.raises(ValueError):
+            be.compound_fprop_distill(**dict(d, temperature=0))
+
+
 def test_the_workspace_grows_and_is_kept(be):
     events = []
     be.rt = NoDevice()
@@ -232,10 +267,10 @@ def test_entry_points_check_arguments_before_they_need_a_device():
     P, BIG = 4096, 1 << 40
     ok = []
     #       y mean var x gamma beta eps  dtype axis F   N  ldx ldy ws bytes stream
-    good = [P, P, P, P, P, P, 1e-5, 0, 0, 2000, 64, 64, 64, P, BIG, None]
+    good = [P, P, P, P, P, P, 1e-5, 0, 0, 5000, 64, 64, 64, P, BIG, None]
     ok.append(codes(lib, "nh_ln_fprop", good, [
         {0: None}, {1: None}, {2: None}, {3: None}, {4: None}, {5: None}, {7: 3}, {7: -1}, {8: 2}, {9: 0}, {9: 1 << 31},
-        {10: 1 << 41}, {11: 63}, {12: 63}, {13: None}, {14: lib.nh_ln_workspace_bytes(0, 0, 0, 2000, 64) - 1}]))
+        {10: 1 << 41}, {11: 63}, {12: 63}, {13: None}, {14: lib.nh_ln_workspace_bytes(0, 0, 0, 5000, 64) - 1}]))
     #       dx dg db dy x mean var gamma eps dtype axis F N ldx lddy lddx ws bytes stream
     good = [P, P, P, P, P, P, P, P, 1e-5, 2, 1, 100, 64, 100, 100, 100, P, BIG, None]
     ok.append(codes(lib, "nh_ln_bprop", good, [

@@ -331,7 +331,7 @@ int nh_embed_update(void* dW, const void* err, const int32_t* ids, float scale, 
  * ids along entries and positions, t along entries and positions, loss along
  * positions, stats along its four values and along positions.                  */
 #define NH_DISTILL_MAX_ENTRIES 1024
-size_t nh_distill_workspace_bytes(int backward, int dtype, int axis, size_t vocab, size_t positions, size_t entries);
+size_t nh_distill_workspace_bytes(int dtype, int axis, size_t vocab, size_t positions);       /* of nh_distill_fprop */
 int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* ids, const void* t,
                      float temperature, int dtype, int t_dtype, int axis, size_t vocab, size_t positions, size_t entries,
                      size_t ld_z, const int64_t* strides, void* workspace, size_t workspace_bytes, void* stream);
@@ -342,7 +342,7 @@ int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* id
 int nh_distill_bprop(void* dz, const void* z, const int32_t* ids, const void* t, const float* stats,
                      const float* weight, float weight_all, float temperature, int dtype, int t_dtype, int axis,
                      size_t vocab, size_t positions, size_t entries, size_t ld_z, size_t ld_dz, const int64_t* strides,
-                     void* workspace, size_t workspace_bytes, void* stream);
+                     void* stream);
 
 #ifdef __cplusplus
 }

@@ -496,7 +496,7 @@ class LanguageModelOps(object):
             if t.take_array:
                 t, _ = self._lm_in(t, axis, layout, temps)
             rt, vocab = self.rt, y.shape[axis]
-            need = rt.lib.nh_distill_workspace_bytes(0, code, layout, vocab, positions, entries)
+            need = rt.lib.nh_distill_workspace_bytes(code, layout, vocab, positions)
             ws, ws_bytes = self._lm_workspace(need)
             strides = hiprt.int64s(ids.strides[axis], ids.strides[1 - axis], t.strides[axis], t.strides[1 - axis],
                                    loss.strides[1 - axis], stats.strides[axis], stats.strides[1 - axis])
@@ -520,12 +520,10 @@ class LanguageModelOps(object):
         key, tail = self._lm_form("distill grad" if tensor_weight else "distill grad, one weight", axis,
                                   (delta, y, ids, t, stats) + ((weight,) if tensor_weight else ()), 1)
         if tail is not None:
-            ws, ws_bytes = self._lm_workspace(tail[9])
             hiprt.check(self.rt.lib.nh_distill_bprop(delta.gpudata, y.gpudata, ids.gpudata, t.gpudata, stats.gpudata,
                                                      weight.gpudata if tensor_weight else None,
                                                      1.0 if tensor_weight else float(weight),
-                                                     self._lm_temperature(temperature), *tail[:9], ws, ws_bytes,
-                                                     self.rt.stream))
+                                                     self._lm_temperature(temperature), *tail, self.rt.stream))
             return
         self._lm_tensors(axis, (delta,), (y, ids, t, stats) + ((weight,) if tensor_weight else ()))
         code, t_code = _storage("y", y), _storage("t", t)
@@ -550,16 +548,13 @@ class LanguageModelOps(object):
             if tensor_weight and weight.take_array:
                 weight = self._lm_vector_in(weight, 1 - axis, temps)
             rt, vocab = self.rt, y.shape[axis]
-            need = rt.lib.nh_distill_workspace_bytes(1, code, layout, vocab, positions, entries)
-            ws, ws_bytes = self._lm_workspace(need)
             strides = hiprt.int64s(ids.strides[axis], ids.strides[1 - axis], t.strides[axis], t.strides[1 - axis],
                                    stats.strides[axis], stats.strides[1 - axis], weight.strides[1 - axis] if tensor_weight else 0)
             tail = (code, t_code, layout, vocab, positions, entries, ld_z, ld_dz, strides)
             hiprt.check(rt.lib.nh_distill_bprop(dz.gpudata, z.gpudata, ids.gpudata, t.gpudata, stats.gpudata,
                                                 weight.gpudata if tensor_weight else None,
-                                                1.0 if tensor_weight else float(weight), temperature, *tail, ws, ws_bytes,
-                                                rt.stream))
-            self._lm_keep(key, temps, tail + (need,))
+                                                1.0 if tensor_weight else float(weight), temperature, *tail, rt.stream))
+            self._lm_keep(key, temps, tail)
             self._lm_copy_back(back)
         finally:
             self._lm_release(temps)

@@ -122,13 +122,13 @@ SIGNATURES = {
     "nh_embed_update_workspace_bytes": (c_size_t, [c_int, c_int, c_size_t, c_size_t, c_size_t]),
     "nh_embed_update": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_float, c_int, c_int, c_size_t, c_size_t,
                                 c_size_t, c_size_t, c_size_t, c_int64, c_void_p, c_size_t, c_void_p]),
-    "nh_distill_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_size_t, c_size_t, c_size_t]),
+    "nh_distill_workspace_bytes": (c_size_t, [c_int, c_int, c_size_t, c_size_t]),
     "nh_distill_fprop": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_int,
                                  c_int, c_size_t, c_size_t, c_size_t, c_size_t, c_void_p, c_void_p, c_size_t,
                                  c_void_p]),
     "nh_distill_bprop": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_float,
                                  c_int, c_int, c_int, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_void_p,
-                                 c_void_p, c_size_t, c_void_p]),
+                                 c_void_p]),
     "nh_colmax_argmax_f32_static": (c_int, [c_void_p, c_void_p, c_void_p, c_uint32, c_uint32,
                                             c_size_t, c_void_p]),
 }

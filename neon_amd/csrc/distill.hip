@@ -42,7 +42,6 @@ struct DistillArgs {
     long long ids_k, ids_n, t_k, t_n;           // strides of the entry tensors
     long long loss_n, stat_n, weight_n;
     nh_pair* part;          // forward: (maximum, sum) per position and chunk
-    uint2* target;          // backward, columns: (word, probability) per entry and position
     uint32_t chunk, chunks;
     bool stream;            // the logits are more than the last-level cache holds: read and written past it
 };
@@ -103,27 +102,42 @@ NEON_DEV Lse lse_wave(Lse v, float c) {
 NEON_DEV float wave_sum(float v) { return nh_wave_allreduce<nh_op_sum, 64>(v); }
 NEON_DEV float wave_max(float v) { return nh_wave_allreduce<nh_op_max, 64>(v); }
 
+// where a position's entries are read from
+struct InMemory {
+    const DistillArgs& a;
+    size_t n;
+    NEON_DEV int id(uint32_t k) const { return load_id(a, k, n); }
+    NEON_DEV float t(uint32_t k) const { return load_t(a, k, n); }
+};
+struct InLds {
+    const int* ids;
+    const float* ts;
+    NEON_DEV int id(uint32_t k) const { return ids[k]; }
+    NEON_DEV float t(uint32_t k) const { return ts[k]; }
+};
+
 // One wave, with the student's state of position n: the teacher's entries, the
 // loss and the statistics.  z[v * step] is the logit of word v.
-template <typename T> NEON_DEV void finish_position(const DistillArgs& a, size_t n, Lse st, const T* z, size_t step) {
+template <typename T, class E>
+NEON_DEV void finish_position(const DistillArgs& a, size_t n, Lse st, const T* z, size_t step, const E& entry) {
     const int lane = threadIdx.x & 63;
     const float log_s = logf(st.s);
     float top = -NH_INF;
     for (uint32_t k = lane; k < a.entries; k += 64)
-        if (is_word(load_id(a, k, n), a.vocab)) top = nh_max(top, load_t(a, k, n));
+        if (is_word(entry.id(k), a.vocab)) top = nh_max(top, entry.t(k));
     top = wave_max(top);
     const bool some = top != -NH_INF;
     const float top0 = some ? top : 0.0f;
     float sum = 0.0f;
     for (uint32_t k = lane; k < a.entries; k += 64)
-        if (is_word(load_id(a, k, n), a.vocab)) sum += expf((load_t(a, k, n) - top0) * a.inv_t);
+        if (is_word(entry.id(k), a.vocab)) sum += expf((entry.t(k) - top0) * a.inv_t);
     sum = wave_sum(sum);
     const float log_t = logf(sum);
     float loss = 0.0f;
     for (uint32_t k = lane; k < a.entries && some; k += 64) {
-        const int id = load_id(a, k, n);
+        const int id = entry.id(k);
         if (!is_word(id, a.vocab)) continue;
-        const float log_p = (load_t(a, k, n) - top0) * a.inv_t - log_t;
+        const float log_p = (entry.t(k) - top0) * a.inv_t - log_t;
         const float p = expf(log_p);
         const float log_q = ((float)z[(size_t)id * step] - st.m) * a.inv_t - log_s;
         if (p != 0.0f) loss = __builtin_fmaf(p, log_p - log_q, loss);
@@ -202,7 +216,7 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_lse_ke
     if (threadIdx.x < 64) {
         st = lse_join(lse_join(slots[0], slots[1], c), lse_join(slots[2], slots[3], c), c);
         if (a.chunks == 1) {
-            finish_position(a, n, st, z, 1);
+            finish_position(a, n, st, z, 1, InMemory{a, n});
             return;
         }
         nh_pair p;
@@ -218,8 +232,9 @@ template <typename T> struct strip { static constexpr int COLS = LC * vec<T>::V;
 template <typename T> __global__ __launch_bounds__(256) void distill_cols_lse_kernel(DistillArgs a) {
     constexpr int V = vec<T>::V, COLS = strip<T>::COLS, RL = 256 / LC, AHEAD = 8;
     __shared__ Lse slots[4][COLS];
-    const size_t c0 = (size_t)(blockIdx.x / a.chunks) * COLS;
-    const uint32_t chunk = blockIdx.x % a.chunks;
+    const uint32_t strips = gridDim.x / a.chunks;        // (neighbouring workgroups: neighbouring memory)
+    const size_t c0 = (size_t)(blockIdx.x % strips) * COLS;
+    const uint32_t chunk = blockIdx.x / strips;
     const uint32_t i0 = chunk * a.chunk, i1 = i0 + a.chunk < a.vocab ? i0 + a.chunk : a.vocab;
     const int cl = threadIdx.x % LC, rl = threadIdx.x / LC;
     const size_t col = c0 + cl * V;
@@ -269,17 +284,35 @@ template <typename T> __global__ __launch_bounds__(256) void distill_cols_lse_ke
     }
 }
 
-// positions whose vocabulary was split, and the columns layout: a wave per position
-template <typename T> __global__ __launch_bounds__(256) void distill_finish_kernel(DistillArgs a, size_t z_n, size_t z_v) {
-    const size_t n = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= a.positions) return;
-    const float c = a.inv_t * LOG2E;
-    Lse st = {-NH_INF, 0.0f};
-    for (uint32_t i = threadIdx.x & 63; i < a.chunks; i += 64) {
-        const nh_pair p = a.part[n * a.chunks + i];
-        st = lse_join(st, {p.v, __builtin_bit_cast(float, p.i)}, c);
+// Positions whose vocabulary was split, and the columns layout: `group` positions
+// per workgroup (a multiple of its four waves), their entries brought to LDS side
+// by side -- in the columns layout an entry's neighbours in memory are other
+// positions', and 16 of them share a cache line.
+template <typename T> __global__ __launch_bounds__(256) void distill_finish_kernel(DistillArgs a, size_t z_n, size_t z_v, bool rows,
+                                                                                  uint32_t group) {
+    extern __shared__ int entries[];          // ids, then t: [position][entry]
+    float* ts = (float*)(entries + group * a.entries);
+    const size_t n0 = (size_t)blockIdx.x * group;
+    const uint32_t all = group * a.entries;
+    for (uint32_t i = threadIdx.x; i < all; i += 256) {
+        const uint32_t x = rows ? i / a.entries : i % group, k = rows ? i % a.entries : i / group;
+        if (n0 + x >= a.positions) continue;
+        entries[x * a.entries + k] = load_id(a, k, n0 + x);
+        ts[x * a.entries + k] = load_t(a, k, n0 + x);
     }
-    finish_position(a, n, lse_wave(st, c), (const T*)a.z + n * z_n, z_v);
+    __syncthreads();
+    const float c = a.inv_t * LOG2E;
+    for (uint32_t x = threadIdx.x >> 6; x < group; x += 4) {
+        const size_t n = n0 + x;
+        if (n >= a.positions) return;
+        Lse st = {-NH_INF, 0.0f};
+        for (uint32_t i = threadIdx.x & 63; i < a.chunks; i += 64) {
+            const nh_pair p = a.part[n * a.chunks + i];
+            st = lse_join(st, {p.v, __builtin_bit_cast(float, p.i)}, c);
+        }
+        finish_position(a, n, lse_wave(st, c), (const T*)a.z + n * z_n, z_v,
+                        InLds{entries + x * a.entries, ts + x * a.entries});
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -292,12 +325,47 @@ NEON_DEV float prob_q(float z, float inv_t, float top, float log_sum) {
     return __builtin_amdgcn_exp2f(__builtin_fmaf(z - top, inv_t, -log_sum) * LOG2E);
 }
 
+// Which of a position's words are named more than once: a table of word ids in
+// LDS with at least twice as many places as entries, open addressing.  Returns
+// the place of `id`; `twice` gets a bit for a place that was asked for again.
+NEON_DEV uint32_t table_size(uint32_t entries) {
+    uint32_t n = 64;
+    while (n < 2 * entries) n *= 2;
+    return n;
+}
+NEON_DEV uint32_t table_put(int* table, uint32_t* twice, uint32_t size, int id) {
+    uint32_t at = ((uint32_t)id * 2654435761u >> 16) & (size - 1);
+    for (;;) {
+        const int old = atomicCAS(&table[at], -1, id);
+        if (old == -1) return at;
+        if (old == id) {
+            atomicOr(&twice[at >> 5], 1u << (at & 31));
+            return at;
+        }
+        at = (at + 1) & (size - 1);
+    }
+}
+// (is entry k the first with its word?, the sum over all of them), for words named more than once
+NEON_DEV bool first_and_sum(const int* ids, const float* ps, uint32_t entries, uint32_t k, float& p) {
+    const int id = ids[k];
+    bool first = true;
+    p = 0.0f;
+    for (uint32_t o = 0; o < entries; ++o)
+        if (ids[o] == id) {
+            first = first && o >= k;
+            p += ps[o];
+        }
+    return first;
+}
+constexpr int MOST_PLACES = 2 * MOST_ENTRIES;
+
 // One workgroup per position and chunk of the vocabulary: w T q over the chunk,
 // then the few words of the chunk that the teacher names once more with p in.
 template <typename T> __global__ __launch_bounds__(256) void distill_rows_bprop_kernel(DistillArgs a) {
     constexpr int V = vec<T>::V, AHEAD = 4;
-    __shared__ int ids[MOST_ENTRIES];
+    __shared__ int ids[MOST_ENTRIES], table[MOST_PLACES];
     __shared__ float ps[MOST_ENTRIES];
+    __shared__ uint32_t twice[MOST_PLACES / 32];
     const size_t n = blockIdx.x / a.chunks;
     const uint32_t i0 = (blockIdx.x % a.chunks) * a.chunk;
     const uint32_t i1 = i0 + a.chunk < a.vocab ? i0 + a.chunk : a.vocab;
@@ -306,10 +374,13 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_bprop_
     const Stats st = load_stats(a, n);
     const bool some = st.t_top != -NH_INF;
     const float w = weight_of(a, n);
+    const uint32_t places = table_size(a.entries);
     for (uint32_t k = threadIdx.x; k < a.entries && some; k += 256) {
         ids[k] = load_id(a, k, n);
         ps[k] = entry_p(a, load_t(a, k, n), st);
     }
+    for (uint32_t k = threadIdx.x; k < places; k += 256) table[k] = -1;
+    if (threadIdx.x < places / 32) twice[threadIdx.x] = 0;
     const auto grad = [&](float x) { return some ? w * prob_q(x, a.inv_t, st.top, st.log_sum) : 0.0f; };
     // batches of AHEAD vectors per thread.  Loads return in the order of issue, stores among them: the
     // next batch is asked for before this one is stored.
@@ -357,111 +428,135 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_bprop_
     }
     if (!some) return;
     __syncthreads();        // the entries are in LDS, and the chunk is written before its words are written again
-    for (uint32_t k = threadIdx.x; k < a.entries; k += 256) {
-        const uint32_t id = (uint32_t)ids[k];
-        if (id < i0 || id >= i1) continue;
-        float p = 0.0f;
-        bool first = true;
-        for (uint32_t o = 0; o < a.entries; ++o)
-            if ((uint32_t)ids[o] == id) {
-                first = first && o >= k;
-                p += ps[o];
-            }
-        if (first) dz[id] = nh_store_cvt<T>::f(w * (prob_q((float)z[id], a.inv_t, st.top, st.log_sum) - p));
+    constexpr int EACH = MOST_ENTRIES / 256;
+    uint32_t place[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const uint32_t k = threadIdx.x + 256 * e;
+        place[e] = ~0u;
+        if (k < a.entries && (uint32_t)ids[k] >= i0 && (uint32_t)ids[k] < i1) place[e] = table_put(table, twice, places, ids[k]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        if (place[e] == ~0u) continue;
+        const uint32_t k = threadIdx.x + 256 * e, id = (uint32_t)ids[k];
+        float p = ps[k];
+        if (((twice[place[e] >> 5] >> (place[e] & 31)) & 1u) && !first_and_sum(ids, ps, a.entries, k, p)) continue;
+        dz[id] = nh_store_cvt<T>::f(w * (prob_q((float)z[id], a.inv_t, st.top, st.log_sum) - p));
     }
 }
 
-// columns: the teacher's distribution with repeated words joined into their
-// first entry -- (word, probability), word = ~0 for an entry that stands for none
-__global__ __launch_bounds__(64) void distill_target_kernel(DistillArgs a) {
-    __shared__ int ids[MOST_ENTRIES];
-    __shared__ float ps[MOST_ENTRIES];
-    const size_t n = blockIdx.x;
-    const Stats st = load_stats(a, n);
-    const bool some = st.t_top != -NH_INF;
-    for (uint32_t k = threadIdx.x; k < a.entries; k += 64) {
-        ids[k] = some ? load_id(a, k, n) : -1;
-        ps[k] = some ? entry_p(a, load_t(a, k, n), st) : 0.0f;
-    }
-    __syncthreads();
-    for (uint32_t k = threadIdx.x; k < a.entries; k += 64) {
-        const int id = ids[k];
-        bool first = is_word(id, a.vocab);
-        float p = 0.0f;
-        if (first)
-            for (uint32_t o = 0; o < a.entries; ++o)
-                if (ids[o] == id) {
-                    first = first && o >= k;
-                    p += ps[o];
-                }
-        a.target[(size_t)k * a.positions + n] = make_uint2(first ? (uint32_t)id : ~0u, __builtin_bit_cast(uint32_t, p));
-    }
-}
+// Columns: w T q everywhere, by strips of 256 bytes of positions and chunks of
+// the vocabulary; distill_patch_kernel writes the teacher's words once more.
+constexpr int BLC = 16;
+template <typename T> struct bstrip { static constexpr int COLS = BLC * vec<T>::V; };
 
 template <typename T> __global__ __launch_bounds__(256) void distill_cols_bprop_kernel(DistillArgs a) {
-    constexpr int V = vec<T>::V, COLS = strip<T>::COLS, RL = 256 / LC, AHEAD = 8;
-    __shared__ float s_top[COLS], s_log[COLS], s_w[COLS];
-    __shared__ bool s_some[COLS];
-    const size_t c0 = (size_t)(blockIdx.x / a.chunks) * COLS;
-    const uint32_t chunk = blockIdx.x % a.chunks;
-    const uint32_t i0 = chunk * a.chunk, i1 = i0 + a.chunk < a.vocab ? i0 + a.chunk : a.vocab;
-    const int cl = threadIdx.x % LC, rl = threadIdx.x / LC;
-    const size_t col = c0 + cl * V;
+    constexpr int V = vec<T>::V, COLS = bstrip<T>::COLS, RL = 256 / BLC, AHEAD = 4;
+    const uint32_t strips = gridDim.x / a.chunks;        // (neighbouring workgroups: neighbouring memory)
+    const size_t c0 = (size_t)(blockIdx.x % strips) * COLS;
+    const uint32_t i0 = blockIdx.x / strips * a.chunk, i1 = i0 + a.chunk < a.vocab ? i0 + a.chunk : a.vocab;
+    const size_t col = c0 + threadIdx.x % BLC * V;
     const int n = col >= a.positions ? 0 : (a.positions - col >= V ? V : (int)(a.positions - col));
-    if (threadIdx.x < COLS) {
-        const size_t x = c0 + threadIdx.x;
-        const bool real = x < a.positions;
-        const Stats st = load_stats(a, real ? x : 0);
-        s_top[threadIdx.x] = st.top;
-        s_log[threadIdx.x] = st.log_sum;
-        s_some[threadIdx.x] = real && st.t_top != -NH_INF;
-        s_w[threadIdx.x] = real ? weight_of(a, x) : 0.0f;
-    }
-    __syncthreads();
+    if (n == 0) return;
     const T* z = (const T*)a.z + col;
     T* dz = (T*)a.dz + col;
     float top[V], log_sum[V], w[V];
     bool some[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        top[j] = s_top[cl * V + j];
-        log_sum[j] = s_log[cl * V + j];
-        w[j] = s_w[cl * V + j];
-        some[j] = s_some[cl * V + j];
+        const size_t x = col + (j < n ? j : 0);
+        const Stats st = load_stats(a, x);
+        top[j] = st.top;
+        log_sum[j] = st.log_sum;
+        some[j] = st.t_top != -NH_INF;
+        w[j] = weight_of(a, x);
     }
-    if (n > 0)
-        for (uint32_t i = i0 + rl; i < i1; i += AHEAD * RL) {
-            nh_raw<T, V> r[AHEAD];
+    // two sets of registers in turn, as in the rows kernel; words behind the chunk's end are its last one again
+    nh_raw<T, V> even[AHEAD], odd[AHEAD];
+    const auto load = [&](nh_raw<T, V> (&r)[AHEAD], uint32_t i) {
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const uint32_t f = i + k * RL;
-                if (f >= i1) r[k].zero();
-                else if (n == V) r[k].load(z + (size_t)f * a.ld_z);
-                else r[k].load_partial(z + (size_t)f * a.ld_z, n);
-            }
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const uint32_t f = i + k * RL;
-                if (f >= i1) continue;
-                nh_out<T, V> o;
-                o.clear();
-#pragma unroll
-                for (int j = 0; j < V; ++j) o.set(j, some[j] ? w[j] * prob_q(r[k].get(j), a.inv_t, top[j], log_sum[j]) : 0.0f);
-                if (n == V) o.store(dz + (size_t)f * a.ld_dz);
-                else o.store_partial(dz + (size_t)f * a.ld_dz, n);
-            }
+        for (int k = 0; k < AHEAD; ++k) {
+            const T* p = z + (size_t)(i + k * RL < i1 ? i + k * RL : i1 - 1) * a.ld_z;
+            if (n == V) load_logits(r[k], p, a.stream);
+            else r[k].load_partial(p, n);
         }
+    };
+    const auto put = [&](const nh_raw<T, V> (&r)[AHEAD], uint32_t i) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const uint32_t f = i + k * RL;
+            if (f >= i1) continue;
+            nh_out<T, V> o;
+            o.clear();
+#pragma unroll
+            for (int j = 0; j < V; ++j) o.set(j, some[j] ? w[j] * prob_q(r[k].get(j), a.inv_t, top[j], log_sum[j]) : 0.0f);
+            T* p = dz + (size_t)f * a.ld_dz;
+            if (n < V) o.store_partial(p, n);
+            else if (a.stream) o.store_stream(p);
+            else o.store(p);
+        }
+    };
+    constexpr uint32_t BATCH = AHEAD * RL;
+    uint32_t i = i0 + threadIdx.x / BLC;
+    if (i < i1) load(even, i);
+    while (i < i1) {
+        if (i + BATCH < i1) load(odd, i + BATCH);
+        put(even, i);
+        i += BATCH;
+        if (i >= i1) break;
+        if (i + BATCH < i1) load(even, i + BATCH);
+        put(odd, i);
+        i += BATCH;
+    }
+}
+
+// Columns, after that: the words the teacher names, with p in.  A workgroup
+// takes eight positions (in memory an entry's neighbours are other positions');
+// a word named twice is its first entry's.
+constexpr int PATCH = 8;
+size_t patch_lds(size_t entries) {
+    size_t places = 64;
+    while (places < 2 * entries) places *= 2;
+    return PATCH * (entries * 8 + places * 4 + places / 8);
+}
+template <typename T> __global__ __launch_bounds__(256) void distill_patch_kernel(DistillArgs a) {
+    extern __shared__ int lds[];
+    const uint32_t places = table_size(a.entries);
+    const int x = threadIdx.x % PATCH;
+    int* ids = lds + x * a.entries;
+    float* ps = (float*)(lds + PATCH * a.entries) + x * a.entries;
+    int* table = lds + 2 * PATCH * a.entries + x * places;
+    uint32_t* twice = (uint32_t*)(lds + 2 * PATCH * a.entries + PATCH * places) + x * (places / 32);
+    const size_t n = (size_t)blockIdx.x * PATCH + x;
+    Stats st = {};
+    if (n < a.positions) st = load_stats(a, n);
+    const bool some = n < a.positions && st.t_top != -NH_INF;
+    const uint32_t k0 = threadIdx.x / PATCH;
+    constexpr uint32_t STEP = 256 / PATCH;
+    for (uint32_t k = k0; k < a.entries; k += STEP) {
+        ids[k] = some ? load_id(a, k, n) : -1;
+        ps[k] = some ? entry_p(a, load_t(a, k, n), st) : 0.0f;
+    }
+    for (uint32_t k = k0; k < places; k += STEP) table[k] = -1;
+    for (uint32_t k = k0; k < places / 32; k += STEP) twice[k] = 0;
     __syncthreads();
-    const T* z0 = (const T*)a.z + c0;
-    T* dz0 = (T*)a.dz + c0;
-    const uint32_t x = threadIdx.x % COLS;
-    if (c0 + x < a.positions)
-        for (uint32_t k = threadIdx.x / COLS; k < a.entries; k += 256 / COLS) {
-            const uint2 e = a.target[(size_t)k * a.positions + c0 + x];
-            if (e.x < i0 || e.x >= i1) continue;
-            const float q = prob_q((float)z0[(size_t)e.x * a.ld_z + x], a.inv_t, s_top[x], s_log[x]);
-            dz0[(size_t)e.x * a.ld_dz + x] = nh_store_cvt<T>::f(s_w[x] * (q - __builtin_bit_cast(float, e.y)));
-        }
+    for (uint32_t k = k0; k < a.entries; k += STEP)
+        if (is_word(ids[k], a.vocab)) table_put(table, twice, places, ids[k]);
+    __syncthreads();
+    if (!some) return;
+    const float w = weight_of(a, n);
+    for (uint32_t k = k0; k < a.entries; k += STEP) {
+        const int id = ids[k];
+        if (!is_word(id, a.vocab)) continue;
+        float p = ps[k];
+        uint32_t at = ((uint32_t)id * 2654435761u >> 16) & (places - 1);
+        while (table[at] != id) at = (at + 1) & (places - 1);
+        if (((twice[at >> 5] >> (at & 31)) & 1u) && !first_and_sum(ids, ps, a.entries, k, p)) continue;
+        const float q = prob_q((float)((const T*)a.z)[(size_t)id * a.ld_z + n], a.inv_t, st.top, st.log_sum);
+        ((T*)a.dz)[(size_t)id * a.ld_dz + n] = nh_store_cvt<T>::f(w * (q - p));
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -473,6 +568,7 @@ constexpr size_t STREAM_BYTES = (size_t)256 << 20;      // what the last-level c
 struct Chunks {
     uint32_t len, count;
 };
+constexpr size_t MAX_CHUNKS = (size_t)1 << 31;
 Chunks split(size_t vocab, size_t lines, size_t wanted, size_t least) {
     size_t n = lm::ceil_div(wanted, lines ? lines : 1);
     const size_t most = lm::ceil_div(vocab, least);
@@ -487,12 +583,14 @@ Chunks fprop_chunks(int dtype, int axis, size_t vocab, size_t positions) {
     return split(vocab, lm::ceil_div(positions, (size_t)128 / lm::item_bytes(dtype)), 1024, 256);
 }
 Chunks bprop_chunks(int dtype, int axis, size_t vocab, size_t positions) {
-    if (axis == 1) return split(vocab, positions, 2048, 4096);
-    return split(vocab, lm::ceil_div(positions, (size_t)128 / lm::item_bytes(dtype)), 1024, 256);
+    // rows: 16 KB of logits each, one batch of loads.  Workgroups that come and go sweep the memory in
+    // order (8192 x 32000 bf16: 205 us); with a row each they stay, and 2048 rows in step with one another
+    // take 235 us.
+    if (axis == 1) return split(vocab, positions, MAX_CHUNKS, 16384 / lm::item_bytes(dtype));
+    return split(vocab, lm::ceil_div(positions, (size_t)256 / lm::item_bytes(dtype)), MAX_CHUNKS, 128);
 }
 
-size_t workspace_bytes(bool backward, int dtype, int axis, size_t vocab, size_t positions, size_t entries) {
-    if (backward) return axis == 0 ? entries * positions * sizeof(uint2) : 0;
+size_t workspace_bytes(int dtype, int axis, size_t vocab, size_t positions) {
     return positions * fprop_chunks(dtype, axis, vocab, positions).count * sizeof(nh_pair);
 }
 
@@ -514,11 +612,10 @@ int check(const char* who, int dtype, int t_dtype, int axis, size_t vocab, size_
 
 extern "C" {
 
-size_t nh_distill_workspace_bytes(int backward, int dtype, int axis, size_t vocab, size_t positions, size_t entries) {
-    if (check("nh_distill_workspace_bytes", dtype, dtype, axis, vocab, positions, entries, 1.0f, axis == 1 ? vocab : positions,
-              axis == 1 ? vocab : positions))
-        return 0;
-    return workspace_bytes(backward != 0, dtype, axis, vocab, positions, entries);
+size_t nh_distill_workspace_bytes(int dtype, int axis, size_t vocab, size_t positions) {
+    const size_t line = axis == 1 ? vocab : positions;
+    if (check("nh_distill_workspace_bytes", dtype, dtype, axis, vocab, positions, 0, 1.0f, line, line)) return 0;
+    return workspace_bytes(dtype, axis, vocab, positions);
 }
 
 int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* ids, const void* t,
@@ -528,7 +625,7 @@ int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* id
     if (int rc = check(who, dtype, t_dtype, axis, vocab, positions, entries, temperature, ld_z, ld_z)) return rc;
     if (positions == 0) return 0;
     if (!loss || !stats || !z || !strides || (entries && (!ids || !t))) return lm::refuse(who, "null pointer");
-    const size_t need = workspace_bytes(false, dtype, axis, vocab, positions, entries);
+    const size_t need = workspace_bytes(dtype, axis, vocab, positions);
     if (!workspace || workspace_bytes_given < need) return lm::refuse(who, "workspace smaller than nh_distill_workspace_bytes");
     if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
     lm::OnDevice here;
@@ -548,24 +645,25 @@ int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* id
         if (blocks > lm::MAX_BLOCKS || positions > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
         if (axis == 1) hipLaunchKernelGGL((distill_rows_lse_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
         else hipLaunchKernelGGL((distill_cols_lse_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-        if (axis == 0 || c.count > 1)
-            hipLaunchKernelGGL((distill_finish_kernel<T>), dim3((unsigned)lm::ceil_div(positions, 4)), dim3(256), 0, s, a,
-                           axis == 1 ? ld_z : (size_t)1, axis == 1 ? (size_t)1 : ld_z);
+        if (axis == 0 || c.count > 1) {
+            // (four positions a wave one after another, or one: 256 positions x 32 entries 4.7 us with one, 11 us
+            // with four; 8192 x 256 110 us with one, 53 us with four)
+            const uint32_t group = positions >= 4096 ? 16 : 4;
+            hipLaunchKernelGGL((distill_finish_kernel<T>), dim3((unsigned)lm::ceil_div(positions, group)), dim3(256),
+                               (unsigned)(group * entries * 8), s, a, axis == 1 ? ld_z : (size_t)1,
+                               axis == 1 ? (size_t)1 : ld_z, axis == 1, group);
+        }
         return lm::launched(who);
     });
 }
 
 int nh_distill_bprop(void* dz, const void* z, const int32_t* ids, const void* t, const float* stats,
                      const float* weight, float weight_all, float temperature, int dtype, int t_dtype, int axis, size_t vocab,
-                     size_t positions, size_t entries, size_t ld_z, size_t ld_dz, const int64_t* strides, void* workspace,
-                     size_t workspace_bytes_given, void* stream) {
+                     size_t positions, size_t entries, size_t ld_z, size_t ld_dz, const int64_t* strides, void* stream) {
     const char* who = "nh_distill_bprop";
     if (int rc = check(who, dtype, t_dtype, axis, vocab, positions, entries, temperature, ld_z, ld_dz)) return rc;
     if (positions == 0) return 0;
     if (!dz || !stats || !z || !strides || (entries && (!ids || !t))) return lm::refuse(who, "null pointer");
-    const size_t need = workspace_bytes(true, dtype, axis, vocab, positions, entries);
-    if (need && (!workspace || workspace_bytes_given < need))
-        return lm::refuse(who, "workspace smaller than nh_distill_workspace_bytes");
     if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
     lm::OnDevice here;
     const Chunks c = bprop_chunks(dtype, axis, vocab, positions);
@@ -576,18 +674,20 @@ int nh_distill_bprop(void* dz, const void* z, const int32_t* ids, const void* t,
     a.vocab = (uint32_t)vocab; a.entries = (uint32_t)entries; a.positions = positions; a.ld_z = ld_z; a.ld_dz = ld_dz;
     a.ids_k = strides[0]; a.ids_n = strides[1]; a.t_k = strides[2]; a.t_n = strides[3]; a.stat_k = strides[4];
     a.stat_n = strides[5]; a.weight_n = strides[6];
-    a.target = (uint2*)workspace; a.chunk = c.len; a.chunks = c.count;
+    a.chunk = c.len; a.chunks = c.count;
     a.stream = 2 * vocab * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
     return lm::by_dtype(dtype, [&](auto v) {
         using T = decltype(v);
         const hipStream_t s = (hipStream_t)stream;
-        const size_t blocks = (axis == 1 ? positions : lm::ceil_div(positions, strip<T>::COLS)) * c.count;
+        const size_t blocks = (axis == 1 ? positions : lm::ceil_div(positions, bstrip<T>::COLS)) * c.count;
         if (blocks > lm::MAX_BLOCKS || positions > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
         if (axis == 1) {
             hipLaunchKernelGGL((distill_rows_bprop_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
         } else {
-            if (entries) hipLaunchKernelGGL(distill_target_kernel, dim3((unsigned)positions), dim3(64), 0, s, a);
             hipLaunchKernelGGL((distill_cols_bprop_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+            if (entries)
+                hipLaunchKernelGGL((distill_patch_kernel<T>), dim3((unsigned)lm::ceil_div(positions, PATCH)), dim3(256),
+                                   (unsigned)patch_lds(entries), s, a);
         }
         return lm::launched(who);
     });

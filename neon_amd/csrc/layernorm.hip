@@ -1006,7 +1006,8 @@ constexpr size_t LONG_ROW_FPROP = 65536;      // features one workgroup's regist
 // features of a row that the backward kernel holds with its parameter sums (16 fp32 features
 // per thread of 1024 spill 61 registers)
 size_t long_row_bprop(int dtype) { return dtype == NH_T_F32 ? 8192 : 16384; }
-constexpr size_t FPROP_THREADS = 2048, BPROP_THREADS = 512;       // per CU, of workgroups that walk over rows
+constexpr size_t FPROP_THREADS = 2048;        // per CU, of workgroups that walk over rows
+constexpr size_t BPROP_BLOCKS = 512;          // workgroups of the backward one, which leave a partial row each
 constexpr size_t BPROP_ROWS = 3;              // rows at least that a workgroup leaves one partial row for
 constexpr size_t STREAM_BYTES = (size_t)256 << 20;           // what the last-level cache holds
 constexpr unsigned LONG_ROW_RUNS = 64;        // row runs per feature strip in ln_rows_params_kernel
@@ -1035,13 +1036,20 @@ unsigned row_blocks(size_t positions, size_t threads, size_t per_cu) {
     const size_t blocks = lm::ceil_div(positions, rows);
     return (unsigned)(blocks < most ? blocks : most);
 }
-// threads per row of the backward kernel: at most 16 features each
-size_t bprop_threads(size_t features) { return features <= 64 * 16 ? 64 : features <= 256 * 16 ? 256 : 1024; }
+// threads per row of the backward kernel: 8 features each (16 where a wave or a whole workgroup takes the row)
+size_t bprop_threads(size_t features) { return features <= 64 * 16 ? 64 : features <= 256 * 8 ? 256 : features <= 512 * 8 ? 512 : 1024; }
+unsigned bprop_blocks(size_t features, size_t positions) {
+    const size_t threads = bprop_threads(features), rows = threads == 64 ? 4 : 1;
+    // (two workgroups of 1024 threads do not fit a CU)
+    const size_t most = threads == 1024 ? BPROP_BLOCKS / 2 : BPROP_BLOCKS;
+    const size_t blocks = lm::ceil_div(positions, rows * BPROP_ROWS);
+    return (unsigned)(blocks < most ? blocks : most);
+}
 
 size_t partial_rows(size_t features, size_t positions, int dtype, bool columns) {
     if (columns) return strips_of(COL_BPROP, dtype, positions);
     if (features > long_row_bprop(dtype)) return positions < LONG_ROW_RUNS ? positions : LONG_ROW_RUNS;
-    return row_blocks(lm::ceil_div(positions, BPROP_ROWS), bprop_threads(features), BPROP_THREADS);
+    return bprop_blocks(features, positions);
 }
 
 size_t column_sum_bytes(const ColLimits& l, size_t features, size_t positions, int dtype) {
@@ -1141,7 +1149,7 @@ template <typename T> int bprop_rows(const LnArgs& a, hipStream_t s) {
     else if (a.features <= 64 * 8) LN_GO(64, 8 / V < 2 ? 1 : 2);
     else if (a.features <= 64 * 16) LN_GO(64, 16 / V);
     else if (a.features <= 256 * 8) LN_GO(256, 8 / V);
-    else if (a.features <= 256 * 16) LN_GO(256, 16 / V);
+    else if (a.features <= 512 * 8) LN_GO(512, 8 / V);
     else if (a.features <= 1024 * 8) LN_GO(1024, 8 / V);
     else if constexpr (sizeof(T) == 2) LN_GO(1024, 16 / V);
 #undef LN_GO

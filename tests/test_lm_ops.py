@@ -655,7 +655,7 @@ def test_captured_and_replayed(hip):
                     stats=be.empty((4, n)), dz=be.empty((vocab, n)))
     need = [lib.nh_ln_workspace_bytes(b, 0, 0, f, n) for b in (0, 1)] + \
         [lib.nh_embed_update_workspace_bytes(0, 0, n, embed, vocab)] + \
-        [lib.nh_distill_workspace_bytes(b, 0, 0, vocab, n, k) for b in (0, 1)]
+        [lib.nh_distill_workspace_bytes(0, 0, vocab, n)]
     scratch = [[be.empty((b // 4 + 1, 1)) for b in need] for _ in range(2)]
     strides, strides_b = hiprt.int64s(n, 1, n, 1, 1, n, 1), hiprt.int64s(n, 1, n, 1, n, 1, 0)
 
@@ -672,7 +672,7 @@ def test_captured_and_replayed(hip):
                 lib.nh_distill_fprop(p["loss"], p["stats"], Z, TI, TT, 2.0, 0, 0, 0, vocab, n, k, n, strides,
                                      w[3][0], w[3][1], s),
                 lib.nh_distill_bprop(p["dz"], Z, TI, TT, p["stats"], None, 1.0, 2.0, 0, 0, 0, vocab, n, k, n, n, strides_b,
-                                     w[4][0], w[4][1], s)):
+                                     s)):
             assert rc == 0, lib.nh_last_error()
     eager, recorded = outputs(), outputs()
     fill()

@@ -292,12 +292,12 @@ def test_entry_points_check_arguments_before_they_need_a_device():
     ok.append(codes(lib, "nh_distill_fprop", good, [
         {0: None}, {1: None}, {2: None}, {3: None}, {4: None}, {5: 0.0}, {5: -1.0}, {5: float("nan")},
         {5: float("inf")}, {5: 1e-40}, {6: 3}, {7: 3}, {8: 2}, {9: 0}, {9: 1 << 31}, {10: 1 << 41}, {11: 1025}, {12: 4},
-        {13: None}, {14: None}, {15: lib.nh_distill_workspace_bytes(0, 0, 0, 90, 5, 3) - 1}]))
+        {13: None}, {14: None}, {15: lib.nh_distill_workspace_bytes(0, 0, 90, 5) - 1}]))
     #       dz z ids t stats w wall T dtype tdtype axis V N K ldz lddz strides ws bytes stream
-    good = [P, P, P, P, P, None, 1.0, 1.0, 0, 2, 0, 90, 5, 3, 5, 5, s, P, BIG, None]
+    good = [P, P, P, P, P, None, 1.0, 1.0, 0, 2, 0, 90, 5, 3, 5, 5, s, None]
     ok.append(codes(lib, "nh_distill_bprop", good, [
         {0: None}, {1: None}, {2: None}, {3: None}, {4: None}, {7: 0.0}, {8: 3}, {9: 3}, {10: 2}, {11: 0},
-        {13: 1025}, {14: 4}, {15: 4}, {16: None}, {17: None}, {18: lib.nh_distill_workspace_bytes(1, 0, 0, 90, 5, 3) - 1}]))
+        {13: 1025}, {14: 4}, {15: 4}, {16: None}]))
     count = ctypes.c_int(0)
     if lib.nh_device_count(ctypes.byref(count)) or not count.value:
         assert ok == [hiprt.NH_ENOTINIT] * 6

@@ -16,7 +16,6 @@ a lookup table's gradient (:2591-2660) and cross-entropy
 follow those.
 """
 import math
-import operator
 
 import numpy as np
 
@@ -63,9 +62,6 @@ def _leading(t, axis, layout):
     if positions <= 1:
         return features
     return step_p if step_p >= features else None
-
-
-_address = operator.itemgetter(0)
 
 
 def _dense(t, axis):
@@ -124,12 +120,12 @@ class LanguageModelOps(object):
                 return key, None
         # (every tensor of a kept form is read and written in place; where two might share memory the
         # long way decides)
-        spans = sorted([(t.gpudata, t) for t in tensors], key=_address)
         end = 0
-        for at, t in spans:
-            if at < end:
+        for low, high in sorted([(t.gpudata, t.gpudata + t.nbytes) if t.is_contiguous else self._lm_byte_span(t)
+                                 for t in tensors]):
+            if low < end:
                 return key, None
-            end = at + (t.nbytes if t.is_contiguous else self._lm_byte_span(t)[1] - at)
+            end = high
         if self._deferred or self._pending:
             self._flush()
         return key, tail
@@ -263,6 +259,7 @@ class LanguageModelOps(object):
         1), xmean and xvar (1, positions); with ``axis=1`` all of them
         transposed.  x and y are float32, float16 or bfloat16 alike, the rest is
         float32.  y may be x."""
+        eps = float(eps)
         key, tail = self._lm_form("ln", axis, (y, xmean, xvar, x, gamma, beta), 3)
         if tail is not None:
             ws, ws_bytes = self._lm_workspace(tail[6])
@@ -307,6 +304,7 @@ class LanguageModelOps(object):
         ``delta_in`` with respect to y and the saved statistics.  Shapes and
         types as there; sums over positions are taken in a fixed order.
         delta_out may be delta_in or x."""
+        eps = float(eps)
         key, tail = self._lm_form("ln grad", axis, (delta_out, grad_gamma, grad_beta, delta_in, x, xmean, xvar, gamma), 3)
         if tail is not None:
             ws, ws_bytes = self._lm_workspace(tail[7])
@@ -367,7 +365,7 @@ class LanguageModelOps(object):
         W.  inputs holds int32 ids, in row-major order whatever its shape; W is
         (vocabulary, embedding size); outputs (embedding size, positions) for
         ``axis=0``, (positions, embedding size) for ``axis=1``."""
-        pad = -1 if pad_idx is None else int(pad_idx)
+        pad, scale = -1 if pad_idx is None else int(pad_idx), float(scale)
         key, tail = self._lm_form("lut", axis, (outputs, inputs, W), 1)
         if tail is not None:
             hiprt.check(self.rt.lib.nh_embed_fprop(outputs.gpudata, W.gpudata, inputs.gpudata, scale, *tail, pad,
@@ -404,7 +402,7 @@ class LanguageModelOps(object):
         do not occur.  ``beta=0`` defines every row of dW, ``beta=1`` adds to it.
         error has the shape outputs had; sums are taken in a fixed order, in
         float32."""
-        pad = -1 if pad_idx is None else int(pad_idx)
+        pad, scale, beta = -1 if pad_idx is None else int(pad_idx), float(scale), float(beta)
         key, tail = self._lm_form("lut grad", axis, (dW, inputs, error), 1)
         if tail is not None:
             ws, ws_bytes = self._lm_workspace(tail[7])

@@ -422,6 +422,15 @@ def test_distillation(hip, n, vocab, k, name):
                 check_distill(run_distill(hip, z, ids, t, weight, tau, axis, how, name, name), z, ids, t, weight, tau, name)
 
 
+@pytest.mark.parametrize("n,vocab,k", [(4100, 70, 9), (4097, 50, 600), (9, 3, 300), (300, 40, 1024), (2, 20000, 1000)])
+def test_distillation_of_many_positions_and_repeated_words(hip, n, vocab, k):
+    """entries of 16 positions at a time; words named once, many times, by every entry"""
+    z, ids, t, weight = distill_inputs(n, vocab, k, F32, F32)
+    ids[1] = vocab - 1
+    for axis in (0, 1):
+        check_distill(run_distill(hip, z, ids, t, weight, 1.0, axis, "plain", F32, F32), z, ids, t, weight, 1.0, F32)
+
+
 @pytest.mark.parametrize("how", ["window", "sparse"])
 @pytest.mark.parametrize("name,t_name", [(F32, F16), (F16, F32), (BF16, F32)])
 def test_distillation_on_views(hip, how, name, t_name):
@@ -541,6 +550,59 @@ def test_distillation_gradient_against_differences(hip):
             # losses of size L are off by some 1e-6 L each
             bound = h * h * (np.abs(v).max(1) ** 3).sum() * 1.5 / 2.0 + 1e-5 * np.abs(up).sum() / h
             assert abs(slope - (delta * v).sum()) <= bound
+
+
+# ---- offsets behind 2^32 bytes and 2^31 elements --------------------------------------------------------
+def test_lines_far_apart(hip):
+    """operands whose lines lie 1.2e9 elements apart in one large allocation"""
+    be, ld, lines, width = hip, 1200000000, 4, 300
+    big = [be.empty((lines, ld), dtype=np.float16) for _ in range(2)]
+
+    def put(k, a):
+        for i in range(lines):
+            be.rt.memcpy_h2d(big[k].gpudata + 2 * (i * ld + 7), np.ascontiguousarray(a[i].astype(np.float16)))
+        return big[k][:, 7:7 + width]
+
+    def got(k):
+        out = np.empty((lines, width), np.float16)
+        be.synchronize()
+        for i in range(lines):
+            be.rt.memcpy_d2h(out[i], big[k].gpudata + 2 * (i * ld + 7))
+        return out.astype(np.float64)
+
+    def plain(a, dtype=np.float16):
+        return be.array(np.ascontiguousarray(a).astype(np.float32), dtype=dtype)
+    for axis in (1, 0):               # lines are positions, then features
+        x, dy, gamma, beta = ln_inputs(lines, width, F16) if axis == 1 else ln_inputs(width, lines, F16)
+        X, D = (a if axis == 1 else a.T for a in (x, dy))
+        one_n = (lines, 1) if axis == 1 else (1, width)
+        g, b, mean, var = vec(be, gamma, axis), vec(be, beta, axis), be.empty(one_n), be.empty(one_n)
+        tx, ty = put(0, X), put(1, X)
+        be.compound_fprop_ln(tx, mean, var, g, b, ty, EPS, axis=axis)
+        y = got(1)
+        dg, db = be.empty(g.shape), be.empty(g.shape)
+        be.compound_bprop_ln(ty, dg, db, plain(D), tx, mean, var, g, EPS, axis=axis)
+        dx = got(1)
+        check_ln([y if axis == 1 else y.T, host(mean, axis), host(var, axis), dx if axis == 1 else dx.T, host(dg, axis),
+                  host(db, axis)], x, dy, gamma, beta, F16)
+    W, err, dW, ids = lut_inputs(lines, width, 50, F16, "outside")
+    ti, out = be.array(ids.reshape(1, -1).astype(np.int32), dtype=np.int32), be.empty((50, width), dtype=np.float16)
+    be.compound_fprop_lut(ti, put(0, W), out, axis=1)
+    be.compound_update_lut(ti, plain(err), put(1, dW), beta=1.0, axis=1)
+    check_lut([host(out, 1), got(1)], W, err, dW, ids, F16, None, 1.0, 1.0)
+    for axis in (1, 0):
+        z, tids, t, weight = distill_inputs(lines, width, 5, F16, F16) if axis == 1 else \
+            distill_inputs(width, lines, 5, F16, F16)
+        n = len(z)
+        Z = z if axis == 1 else z.T
+        tt, loss = plain(t if axis == 1 else t.T), be.empty((n, 1) if axis == 1 else (1, n))
+        td = be.array(np.ascontiguousarray(tids if axis == 1 else tids.T).astype(np.int32), dtype=np.int32)
+        stats = be.empty((n, 4) if axis == 1 else (4, n))
+        tz, delta = put(0, Z), put(1, Z)
+        be.compound_fprop_distill(tz, td, tt, loss, stats, axis=axis)
+        be.compound_bprop_distill(delta, tz, td, tt, stats, vec(be, weight, axis), axis=axis)
+        d = got(1)
+        check_distill([host(loss, axis), host(stats, axis), d if axis == 1 else d.T], z, tids, t, weight, 1.0, F16)
 
 
 # ---- in a row, as they are used ------------------------------------------------------------------------

@@ -231,6 +231,15 @@ def test_a_call_of_a_form_seen_before_is_checked_where_it_can_differ(be):
             be.compound_fprop_ln(**dict(b, x=T(be, b["x"].shape, np.float16)))
         with pytest.raises(ValueError):
             be.compound_fprop_ln(**dict(b, axis=1 - axis))
+    # a reversed view lies below its first element
+    d = distill_args(be)
+    d["ids"] = T(be, (3, 4), np.int32, strides=(-4, 1), at=d["ids"].gpudata + 32)
+    be.compound_fprop_distill(**d)
+    be.rt.calls = []
+    be.compound_fprop_distill(**d)
+    assert [c[0] for c in be.rt.calls] == ["nh_distill_fprop"]
+    with pytest.raises(ValueError):
+        be.compound_fprop_distill(**dict(d, loss=T(be, (1, 4), at=d["ids"].gpudata - 32)))
     d = distill_args(be)
     for _ in range(2):
         be.compound_fprop_distill(**d)

@@ -161,7 +161,9 @@ template <typename T, int V> NEON_DEV void load_logits(nh_raw<T, V>& r, const T*
 // ---------------------------------------------------------------------------
 // forward: (maximum, sum) of chunks of the vocabulary.  A position whose
 // vocabulary is one chunk is finished by the same workgroup; otherwise one wave
-// per position joins the chunks in order.
+// per position joins the chunks in order.  4096 x 50001 bf16, 410 MB: 88 us (4.6
+// TB/s), about half of that time in the exponentials; in chunks of 16 KB 102 us, the
+// fold over the lanes being paid for each.
 // ---------------------------------------------------------------------------
 template <typename T> __global__ __launch_bounds__(256) void distill_rows_lse_kernel(DistillArgs a) {
     constexpr int V = vec<T>::V, AHEAD = 4;
@@ -449,6 +451,9 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_bprop_
 
 // Columns: w T q everywhere, by strips of 256 bytes of positions and chunks of
 // the vocabulary; distill_patch_kernel writes the teacher's words once more.
+// 20828 x 9950 fp16, 829 MB: 267 us (3.1 TB/s).  Neighbouring workgroups take
+// neighbouring strips of the same words; with neighbouring chunks of one strip 346
+// us.
 constexpr int BLC = 16;
 template <typename T> struct bstrip { static constexpr int COLS = BLC * vec<T>::V; };
 
@@ -579,6 +584,7 @@ Chunks split(size_t vocab, size_t lines, size_t wanted, size_t least) {
 }
 
 Chunks fprop_chunks(int dtype, int axis, size_t vocab, size_t positions) {
+    // (1024 to 8192 workgroups make no difference in columns: 32000 x 8192 bf16 238 to 243 us, with the finish)
     if (axis == 1) return split(vocab, positions, 1024, 4096);
     return split(vocab, lm::ceil_div(positions, (size_t)128 / lm::item_bytes(dtype)), 1024, 256);
 }
@@ -587,6 +593,7 @@ Chunks bprop_chunks(int dtype, int axis, size_t vocab, size_t positions) {
     // order (8192 x 32000 bf16: 205 us); with a row each they stay, and 2048 rows in step with one another
     // take 235 us.
     if (axis == 1) return split(vocab, positions, MAX_CHUNKS, 16384 / lm::item_bytes(dtype));
+    // columns: 128 words, two batches (20828 x 9950 fp16: 274 us, 256 words 280, 512 words 302)
     return split(vocab, lm::ceil_div(positions, (size_t)256 / lm::item_bytes(dtype)), MAX_CHUNKS, 128);
 }
 

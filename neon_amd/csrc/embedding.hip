@@ -19,7 +19,9 @@
 //                         further workgroups clear (or scale) the rows of absent words
 //   4. lut_join_kernel    adds the partial sums of every word that crosses the end of a run
 // A frequent word (a tenth of all positions in ordinary text) is spread over as
-// many waves as it fills runs.
+// many waves as it fills runs.  32768 positions, 50000 x 1024 bf16: 6 + 8 + 36 + 6
+// us, of which 31 us are the bytes (the errors once, the table once); 1 and 2 and 4
+// wait for memory a few times in a row, whatever they move.
 #include <type_traits>
 
 #include "lm_ops.h"
@@ -33,7 +35,8 @@ constexpr uint32_t NO_WORD = 0xFFFFFFFFu;
 NEON_DEV bool in_table(uint32_t w, uint32_t vocab, uint32_t pad) { return w < vocab && w != pad; }
 
 // ---------------------------------------------------------------------------
-// forward, a position's values side by side: a group of 2^tpr_log threads per position
+// forward, a position's values side by side: a group of 2^tpr_log threads per
+// position.  Bound by HBM and the caches that hold the frequent rows.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void lut_rows_fprop_kernel(T* out, const T* W, const int32_t* ids, float scale, size_t count,
@@ -63,6 +66,7 @@ __global__ __launch_bounds__(256) void lut_rows_fprop_kernel(T* out, const T* W,
 }
 
 // forward, positions side by side: tiles of 128 positions and 128 bytes of columns, turned in LDS
+// (16384 positions x 1024 fp16: 11.5 us, 67 MB, 5.8 TB/s)
 constexpr int TURN_POS = 128;
 template <typename T>
 __global__ __launch_bounds__(256) void lut_cols_fprop_kernel(T* out, const T* W, const int32_t* ids, float scale, size_t count,
@@ -468,7 +472,7 @@ template <typename T> NEON_DEV void clear_rows(const SumArgs& a, uint32_t block)
 // in flight together), and an entry in the
 // list of the waves or of the workgroups of lut_join_kernel.  The order of the
 // lists is any, what becomes of their entries is not.
-constexpr uint32_t MANY_RUNS = 24;
+constexpr uint32_t MANY_RUNS = 24;        // (three rounds of eight loads for a wave)
 template <int RUN> NEON_DEV void list_words(const SumArgs& a, uint32_t total) {
     const size_t run = (size_t)blockIdx.x * 256 + threadIdx.x;
     const size_t s0 = run * RUN;
@@ -539,7 +543,7 @@ template <typename T, int RUN> __global__ __launch_bounds__(256) void lut_sum_ke
     float acc[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) acc[k] = 0.0f;
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = 8;          // (16: 37.6 us instead of 36.3 for 32768 x 1024 bf16)
     for (int i0 = 0; i0 < len; i0 += AHEAD) {
         nh_raw<T, V> r[AHEAD];
 #pragma unroll
@@ -647,7 +651,9 @@ struct Layout {
     int run;              // sorted positions per wave of lut_sum_kernel
 };
 
-// waves of lut_sum_kernel below which it takes shorter runs
+// Waves of lut_sum_kernel below which it takes shorter runs: eight per CU.  32768 x 1024 bf16 takes 37 us in
+// runs of 32 (2048 waves), 42 in runs of 16, whose partial sums are twice as many; 16384 x 300 fp32 takes
+// 20 us in runs of 32 (1024 waves), 15 in runs of 16, 16 in runs of 8.
 constexpr size_t SUM_WAVES = 2048;
 
 Layout layout(int dtype, int axis, size_t count, size_t embed, size_t vocab) {

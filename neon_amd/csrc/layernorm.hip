@@ -100,7 +100,8 @@ template <int TPR> struct RowShape {
 // for before this one is summed up: loads return in the order of issue, stores
 // among them, so a load behind this row's stores would wait for them.  The rows
 // take turns in two sets of registers; moving the next row into this one's place
-// would wait for it.
+// would wait for it.  Bound by HBM: 16384 x 5000 bf16, 328 MB in 66 us (5.0 TB/s; a
+// workgroup per row 84 us, one set of registers 76 us).
 // ---------------------------------------------------------------------------
 template <typename T, int TPR, int NV> __global__ __launch_bounds__(RowShape<TPR>::NT) void ln_rows_fprop_kernel(LnArgs a) {
     constexpr int V = vec<T>::V, RPB = RowShape<TPR>::RPB;
@@ -288,7 +289,9 @@ template <typename T> __global__ __launch_bounds__(1024) void ln_rows_fprop_long
 // rows, backward: a workgroup walks over rows with a fixed set of features per
 // thread, so the sums over positions for dgamma and dbeta stay in registers;
 // each workgroup leaves one partial row of both (gridDim.x of them), which
-// ln_param_kernel adds up in a fixed order.
+// ln_param_kernel adds up in a fixed order.  Bound by HBM: 16384 x 2048 bf16, 201
+// MB in 44 us (4.6 TB/s).  Rows that do not begin on 16 bytes cost about 1.7 times
+// that per byte (7764 x 3356: 2.5 TB/s).
 // ---------------------------------------------------------------------------
 template <typename T, int TPR, int NV> __global__ __launch_bounds__(RowShape<TPR>::NT) void ln_rows_bprop_kernel(LnArgs a) {
     constexpr int V = vec<T>::V, RPB = RowShape<TPR>::RPB;
@@ -492,7 +495,8 @@ template <typename T> __global__ __launch_bounds__(64) void ln_rows_params_kerne
 }
 
 // grads[which][f] = sum of `count` partial rows, in a fixed order: 128 threads
-// per 4 features take every 128th row, joined in LDS
+// per 4 features take every 128th row, joined in LDS.  Latency: 784 rows of 2 x 1024
+// in 5 us (one thread per feature and 16th of the rows: 16 us).
 __global__ __launch_bounds__(1024) void ln_param_kernel(LnArgs a, uint32_t count) {
     __shared__ float join[128][36];
     const int lane = threadIdx.x & 7, grp = threadIdx.x >> 3;
@@ -703,6 +707,7 @@ template <typename T, int NT, int LC, int RV> struct ColFprop {
 
 // The features of a strip in registers: x is read once.  Loads return in the
 // order of issue, stores among them, so gamma and beta are asked for first.
+// 1024 x 25088 fp16, 103 MB: 31 us (3.3 TB/s); in the two-pass form below 33-39 us.
 template <typename T, int NT, int LC, int RV> __global__ __launch_bounds__(NT, 4) void ln_cols_fprop_kernel(LnArgs a) {
     using K = ColFprop<T, NT, LC, RV>;
     __shared__ typename K::Shared m;
@@ -904,7 +909,10 @@ template <typename T, int NT> struct ColBprop {
 // Loads return in the order of issue, stores among them: what is small (the
 // statistics, gamma) is asked for first, the features' sums go through LDS and
 // are stored last, so that the additions of a feature wait for its own two loads
-// only.
+// only.  1024 x 25088 fp16, 154 MB: 53 us (2.9 TB/s); with gamma read where it is
+// used and the sums stored at once 65 us, with both tensors streamed twice 58-60
+// us.  What is left: 784 strips on 512 places, and lines of 50 KB of which a strip
+// reads 64 bytes.
 template <typename T, int NT, int RV> __global__ __launch_bounds__(NT, 4) void ln_cols_bprop_kernel(LnArgs a) {
     using K = ColBprop<T, NT>;
     __shared__ typename K::Shared m;
@@ -1006,9 +1014,15 @@ constexpr size_t LONG_ROW_FPROP = 65536;      // features one workgroup's regist
 // features of a row that the backward kernel holds with its parameter sums (16 fp32 features
 // per thread of 1024 spill 61 registers)
 size_t long_row_bprop(int dtype) { return dtype == NH_T_F32 ? 8192 : 16384; }
-constexpr size_t FPROP_THREADS = 2048;        // per CU, of workgroups that walk over rows
-constexpr size_t BPROP_BLOCKS = 512;          // workgroups of the backward one, which leave a partial row each
-constexpr size_t BPROP_ROWS = 3;              // rows at least that a workgroup leaves one partial row for
+// Workgroups that walk over rows.  Forward, threads per CU: 16384 x 5000 bf16 takes 73.4 us with 1024,
+// 73.0 with 2048, 74.6 with 3072 (and 126 with 512, when too few rows are in flight).  Backward, where every
+// workgroup leaves a partial row of both parameter sums: 16384 x 2048 bf16 takes 57 us with 256
+// workgroups, 43 with 512, 46 with 1024, 56 with 2048.
+constexpr size_t FPROP_THREADS = 2048;
+constexpr size_t BPROP_BLOCKS = 512;
+// Rows at least that a workgroup leaves one partial row for (777 x 1537 fp32: 10.5 + 3.7 us with one or two
+// rows each, 8.6 + 2.5 us with three).
+constexpr size_t BPROP_ROWS = 3;
 constexpr size_t STREAM_BYTES = (size_t)256 << 20;           // what the last-level cache holds
 constexpr unsigned LONG_ROW_RUNS = 64;        // row runs per feature strip in ln_rows_params_kernel
 constexpr size_t COL_CHUNKS = 32;             // runs of tiles per strip of a split column kernel, at most
@@ -1036,7 +1050,9 @@ unsigned row_blocks(size_t positions, size_t threads, size_t per_cu) {
     const size_t blocks = lm::ceil_div(positions, rows);
     return (unsigned)(blocks < most ? blocks : most);
 }
-// threads per row of the backward kernel: 8 features each (16 where a wave or a whole workgroup takes the row)
+// Threads per row of the backward kernel: 8 features each (16 where a wave or a whole workgroup takes the
+// row).  8000 x 4000 fp32 80 us, 8903 x 5610 bf16 109 us; with 16 each on half the threads, 165 registers
+// leave two workgroups per CU and the latter took 181 us.
 size_t bprop_threads(size_t features) { return features <= 64 * 16 ? 64 : features <= 256 * 8 ? 256 : features <= 512 * 8 ? 512 : 1024; }
 unsigned bprop_blocks(size_t features, size_t positions) {
     const size_t threads = bprop_threads(features), rows = threads == 64 ? 4 : 1;

@@ -286,9 +286,9 @@ int nh_lut_bprop(void* dW, const void* error_t, const int32_t* ids, int itemsize
  * position's values lie along in a row-major matrix: 1 = (positions, features),
  * 0 = (features, positions).  Leading dimensions are elements between stored
  * lines; the lines themselves are dense and may start at any element.
- * Workspaces are device scratch, need not be initialised, and belong to one
- * call at a time: calls that may overlap (other streams, captured graphs) need
- * one each.  No call allocates, synchronises or records a memset.  Arguments
+ * Workspaces are device scratch on a 16-byte boundary, need not be
+ * initialised, and belong to one call at a time: calls that may overlap (other
+ * streams, captured graphs) need one each.  No call allocates, synchronises or records a memset.  Arguments
  * are checked before anything is launched.  The kernels run on the device of
  * nh_init.                                                                     */
 #define NH_T_F32 0

@@ -634,6 +634,7 @@ int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* id
     if (!loss || !stats || !z || !strides || (entries && (!ids || !t))) return lm::refuse(who, "null pointer");
     const size_t need = workspace_bytes(dtype, axis, vocab, positions);
     if (!workspace || workspace_bytes_given < need) return lm::refuse(who, "workspace smaller than nh_distill_workspace_bytes");
+    if (!lm::aligned16(workspace)) return lm::refuse(who, "workspace off a 16-byte boundary");
     if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
     lm::OnDevice here;
     const Chunks c = fprop_chunks(dtype, axis, vocab, positions);

@@ -742,6 +742,7 @@ int nh_embed_update(void* dW, const void* err, const int32_t* ids, float scale, 
     if (!dW || (positions && (!err || !ids))) return lm::refuse(who, "null pointer");
     const Layout l = layout(dtype, axis, positions, embed, vocab);
     if (!workspace || workspace_bytes < l.bytes) return lm::refuse(who, "workspace smaller than nh_embed_update_workspace_bytes");
+    if (!lm::aligned16(workspace)) return lm::refuse(who, "workspace off a 16-byte boundary");
     if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
     lm::OnDevice here;
     const hipStream_t s = (hipStream_t)stream;

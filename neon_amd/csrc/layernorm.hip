@@ -1212,6 +1212,7 @@ int nh_ln_fprop(void* y, float* mean, float* var, const void* x, const float* ga
     const size_t need = workspace_bytes(false, dtype, axis == 0, features, positions);
     if (need && (!workspace || workspace_bytes_given < need))
         return lm::refuse("nh_ln_fprop", "workspace smaller than nh_ln_workspace_bytes");
+    if (!lm::aligned16(workspace)) return lm::refuse("nh_ln_fprop", "workspace off a 16-byte boundary");
     if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
     lm::OnDevice here;
     LnArgs a = {};
@@ -1233,6 +1234,7 @@ int nh_ln_bprop(void* dx, float* dgamma, float* dbeta, const void* dy, const voi
     const size_t need = workspace_bytes(true, dtype, axis == 0, features, positions);
     if (need && (!workspace || workspace_bytes_given < need))
         return lm::refuse("nh_ln_bprop", "workspace smaller than nh_ln_workspace_bytes");
+    if (!lm::aligned16(workspace)) return lm::refuse("nh_ln_bprop", "workspace off a 16-byte boundary");
     if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
     lm::OnDevice here;
     LnArgs a = {};

@@ -27,6 +27,8 @@ inline size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
 inline int item_bytes(int dtype) { return dtype == NH_T_F32 ? 4 : 2; }
 inline bool known_dtype(int dtype) { return dtype == NH_T_F32 || dtype == NH_T_F16 || dtype == NH_T_BF16; }
 
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
 inline int refuse(const char* who, const char* why) {
     return nh_internal_fail(NH_EINVAL, (std::string(who) + ": " + why).c_str());
 }

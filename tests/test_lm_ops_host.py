@@ -279,12 +279,12 @@ def test_entry_points_check_arguments_before_they_need_a_device():
     good = [P, P, P, P, P, P, 1e-5, 0, 0, 5000, 64, 64, 64, P, BIG, None]
     ok.append(codes(lib, "nh_ln_fprop", good, [
         {0: None}, {1: None}, {2: None}, {3: None}, {4: None}, {5: None}, {7: 3}, {7: -1}, {8: 2}, {9: 0}, {9: 1 << 31},
-        {10: 1 << 41}, {11: 63}, {12: 63}, {13: None}, {14: lib.nh_ln_workspace_bytes(0, 0, 0, 5000, 64) - 1}]))
+        {10: 1 << 41}, {11: 63}, {12: 63}, {13: None}, {13: P + 8}, {14: lib.nh_ln_workspace_bytes(0, 0, 0, 5000, 64) - 1}]))
     #       dx dg db dy x mean var gamma eps dtype axis F N ldx lddy lddx ws bytes stream
     good = [P, P, P, P, P, P, P, P, 1e-5, 2, 1, 100, 64, 100, 100, 100, P, BIG, None]
     ok.append(codes(lib, "nh_ln_bprop", good, [
         {0: None}, {1: None}, {2: None}, {3: None}, {4: None}, {5: None}, {6: None}, {7: None}, {9: 9}, {10: 5}, {11: 0},
-        {13: 99}, {14: 99}, {15: 99}, {16: None}, {17: lib.nh_ln_workspace_bytes(1, 2, 1, 100, 64) - 1}]))
+        {13: 99}, {14: 99}, {15: 99}, {16: None}, {16: P + 4}, {17: lib.nh_ln_workspace_bytes(1, 2, 1, 100, 64) - 1}]))
     #       out W ids scale dtype axis N E V ldw ldout pad stream
     good = [P, P, P, 1.0, 1, 0, 50, 20, 30, 20, 50, -1, None]
     ok.append(codes(lib, "nh_embed_fprop", good, [
@@ -293,7 +293,7 @@ def test_entry_points_check_arguments_before_they_need_a_device():
     #       dW err ids scale beta dtype axis N E V lddw lderr pad ws bytes stream
     good = [P, P, P, 1.0, 0.0, 1, 1, 50, 20, 30, 20, 20, -1, P, BIG, None]
     ok.append(codes(lib, "nh_embed_update", good, [
-        {0: None}, {1: None}, {2: None}, {5: 7}, {6: 2}, {7: 1 << 31}, {8: 0}, {9: 0}, {10: 19}, {11: 19}, {13: None},
+        {0: None}, {1: None}, {2: None}, {5: 7}, {6: 2}, {7: 1 << 31}, {8: 0}, {9: 0}, {10: 19}, {11: 19}, {13: None}, {13: P + 8},
         {14: lib.nh_embed_update_workspace_bytes(1, 1, 50, 20, 30) - 1}]))
     s = hiprt.int64s(5, 1, 5, 1, 1, 5, 1)
     #       loss stats z ids t T dtype tdtype axis V N K ldz strides ws bytes stream
@@ -301,7 +301,7 @@ def test_entry_points_check_arguments_before_they_need_a_device():
     ok.append(codes(lib, "nh_distill_fprop", good, [
         {0: None}, {1: None}, {2: None}, {3: None}, {4: None}, {5: 0.0}, {5: -1.0}, {5: float("nan")},
         {5: float("inf")}, {5: 1e-40}, {6: 3}, {7: 3}, {8: 2}, {9: 0}, {9: 1 << 31}, {10: 1 << 41}, {11: 1025}, {12: 4},
-        {13: None}, {14: None}, {15: lib.nh_distill_workspace_bytes(0, 0, 90, 5) - 1}]))
+        {13: None}, {14: None}, {14: P + 8}, {15: lib.nh_distill_workspace_bytes(0, 0, 90, 5) - 1}]))
     #       dz z ids t stats w wall T dtype tdtype axis V N K ldz lddz strides ws bytes stream
     good = [P, P, P, P, P, None, 1.0, 1.0, 0, 2, 0, 90, 5, 3, 5, 5, s, None]
     ok.append(codes(lib, "nh_distill_bprop", good, [

@@ -1010,7 +1010,10 @@ template <typename T> __global__ __launch_bounds__(256) void ln_cols_bprop_finis
 // ---------------------------------------------------------------------------
 // launch geometry
 // ---------------------------------------------------------------------------
-constexpr size_t LONG_ROW_FPROP = 65536;      // features one workgroup's registers hold
+// features one workgroup's registers hold; with twice as many fp32 ones 20 registers spill, and
+// the three sweeps are as fast or faster over most of that range: 200 x 33000 17.3 us against
+// 21.4, 2000 x 40000 197 against 216, 5000 x 50000 592 both, 1000 x 65536 168 against 156
+size_t long_row_fprop(int dtype) { return dtype == NH_T_F32 ? 32768 : 65536; }
 // features of a row that the backward kernel holds with its parameter sums (16 fp32 features
 // per thread of 1024 spill 61 registers)
 size_t long_row_bprop(int dtype) { return dtype == NH_T_F32 ? 8192 : 16384; }
@@ -1098,7 +1101,7 @@ template <typename T> int fprop_rows(const LnArgs& a, hipStream_t s) {
     constexpr size_t V = vec<T>::V;
     const size_t nvec = lm::ceil_div(a.features, V);
     if (a.positions > lm::MAX_BLOCKS) return lm::refuse("nh_ln_fprop", "too many positions for one launch");
-    if (a.features > LONG_ROW_FPROP) {
+    if (a.features > long_row_fprop(code_of<T>())) {
         hipLaunchKernelGGL((ln_rows_fprop_long_kernel<T>), dim3((unsigned)a.positions), dim3(1024), 0, s, a);
         return lm::launched("nh_ln_fprop");
     }
@@ -1111,8 +1114,7 @@ template <typename T> int fprop_rows(const LnArgs& a, hipStream_t s) {
     else if (nvec <= 1024) LN_GO(512, 2);
     else if (nvec <= 2048) LN_GO(1024, 2);
     else if (nvec <= 4096) LN_WIDE(4);
-    else if (nvec <= 8192) LN_WIDE(8);
-    else if constexpr (sizeof(T) == 4) LN_WIDE(16);
+    else LN_WIDE(8);
 #undef LN_WIDE
 #undef LN_GO
     return lm::launched("nh_ln_fprop");

@@ -3,6 +3,10 @@ the backend's methods on tensors with made-up addresses, and the C entry points
 called directly (they check arguments before they need a device).  Also the
 float64 formulas the GPU tests compare with, against differences."""
 import ctypes
+import os
+import re
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -12,6 +16,9 @@ import neon_amd.backends  # noqa: F401
 from neon_amd.backends import HIPTensor, NervanaHIP, bfloat16
 from neon_amd.backends.hip import lmops
 from neon_amd.backends.hip import runtime as hiprt
+
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 class NoDevice(object):
@@ -315,6 +322,24 @@ def test_entry_points_check_arguments_before_they_need_a_device():
 test_entry_points_check_arguments_before_they_need_a_device = pytest.mark.skipif(
     hiprt.device_count() > 0, reason="a device is there: the good calls above would run on made-up addresses")(
         test_entry_points_check_arguments_before_they_need_a_device)
+
+
+# ---- registers ------------------------------------------------------------------------------------
+@pytest.mark.skipif(shutil.which("hipcc") is None, reason="hipcc not on PATH")
+@pytest.mark.parametrize("source", ["layernorm", "embedding", "distill"])
+def test_kernels_keep_to_their_registers(source):
+    """tensors held in registers that spilled would still give the right values,
+    two or three times slower; a few registers' worth of scratch is let pass"""
+    cmd = ["hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang",
+           "-packed-fp32-ops", "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(ROOT, "neon_amd", "csrc"), "-c",
+           os.path.join(ROOT, "neon_amd", "csrc", source + ".hip"), "-o", os.devnull, "--offload-device-only",
+           "-Rpass-analysis=kernel-resource-usage"]
+    out = subprocess.run(cmd, capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr[-2000:]
+    names = re.findall(r"Function Name: (\S+)", out.stderr)
+    scratch = [int(v) for v in re.findall(r"ScratchSize \[bytes/lane\]: (\d+)", out.stderr)]
+    assert len(names) == len(scratch) >= 10
+    assert not [(n, s) for n, s in zip(names, scratch) if s > 16]
 
 
 # ---- the formulas themselves ---------------------------------------------------------------------

@@ -288,9 +288,9 @@ int nh_lut_bprop(void* dW, const void* error_t, const int32_t* ids, int itemsize
  * lines; the lines themselves are dense and may start at any element.
  * Workspaces are device scratch on a 16-byte boundary, need not be
  * initialised, and belong to one call at a time: calls that may overlap (other
- * streams, captured graphs) need one each.  No call allocates, synchronises or records a memset.  Arguments
- * are checked before anything is launched.  The kernels run on the device of
- * nh_init.                                                                     */
+ * streams, captured graphs) need one each.  No call allocates, synchronises or
+ * records a memset.  Arguments are checked before anything is launched.  The
+ * kernels run on the device of nh_init.                                        */
 #define NH_T_F32 0
 #define NH_T_F16 1
 #define NH_T_BF16 2
@@ -327,7 +327,8 @@ int nh_embed_update(void* dW, const void* err, const int32_t* ids, float scale, 
  *   loss = temperature^2 * sum_k p_k (log p_k - log q[id_k])
  * stats: four values per position for the backward pass -- the largest z and
  * log sum_v exp((z_v - largest) / temperature), and the same of the entries' t.
- * No entry (or only t = -inf): loss 0, largest t -inf.  `strides`, in elements:
+ * No entry (or only t = -inf): loss 0, largest t -inf.  The temperature lies
+ * between 2^-60 and 2^60.  `strides`, in elements:
  * ids along entries and positions, t along entries and positions, loss along
  * positions, stats along its four values and along positions.                  */
 #define NH_DISTILL_MAX_ENTRIES 1024

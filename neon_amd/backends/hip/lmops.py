@@ -15,8 +15,6 @@ a lookup table's gradient (:2591-2660) and cross-entropy
 (neon/transforms/cost.py:112-173) in these places; the calling conventions
 follow those.
 """
-import math
-
 import numpy as np
 
 from neon_amd.backends.hip import bf16
@@ -448,8 +446,8 @@ class LanguageModelOps(object):
 
     def _lm_temperature(self, temperature):
         temperature = float(temperature)
-        if not (temperature > 0 and math.isfinite(temperature)):
-            raise ValueError("the temperature is a positive number, not %r" % temperature)
+        if not 2.0 ** -60 <= temperature <= 2.0 ** 60:
+            raise ValueError("the temperature lies between 2**-60 and 2**60, not %r" % temperature)
         return temperature
 
     def compound_fprop_distill(self, y, ids, t, loss, stats, temperature=1.0, axis=0):
@@ -470,7 +468,8 @@ class LanguageModelOps(object):
         With ``axis=0``: y (vocabulary, positions), ids (int32) and t (entries,
         positions), loss (1, positions), stats (4, positions); with ``axis=1``
         all of them transposed.  y and t are float32, float16 or bfloat16, loss
-        and stats float32; at most 1024 entries."""
+        and stats float32; at most 1024 entries, a temperature between 2**-60
+        and 2**60."""
         key, tail = self._lm_form("distill", axis, (loss, stats, y, ids, t), 2)
         if tail is not None:
             ws, ws_bytes = self._lm_workspace(tail[8])

@@ -608,8 +608,9 @@ int check(const char* who, int dtype, int t_dtype, int axis, size_t vocab, size_
     if (vocab == 0 || vocab > 0x7FFFFFFF - 65536) return lm::refuse(who, "between 1 and 2^31 - 65537 words");
     if (positions > (size_t)1 << 40) return lm::refuse(who, "more than 2^40 positions");
     if (entries > MOST_ENTRIES) return lm::refuse(who, "more than NH_DISTILL_MAX_ENTRIES entries per position");
-    if (!(temperature > 0.0f) || !(1.0f / temperature > 0.0f) || temperature > NH_FLT_MAX || 1.0f / temperature > NH_FLT_MAX)
-        return lm::refuse(who, "the temperature is a positive finite number");
+    // (its square multiplies the loss, and its inverse's product with log2(e) the logits: both finite, neither 0)
+    if (!(temperature >= 0x1p-60f && temperature <= 0x1p60f))
+        return lm::refuse(who, "the temperature lies between 2^-60 and 2^60");
     const size_t len = axis == 1 ? vocab : positions, lines = axis == 1 ? positions : vocab;
     if (lines > 1 && (ld_a < len || ld_b < len)) return lm::refuse(who, "leading dimension shorter than a line");
     return 0;

@@ -193,6 +193,7 @@ def test_embedding_refusals(be):
 def test_distillation_refusals(be):
     for bad, error in ((dict(temperature=0.0), ValueError), (dict(temperature=-1), ValueError),
                        (dict(temperature=float("nan")), ValueError), (dict(temperature=float("inf")), ValueError),
+                       (dict(temperature=1e20), ValueError), (dict(temperature=1e-20), ValueError),
                        (dict(ids=T(be, (3, 4))), TypeError), (dict(ids=T(be, (3, 5), np.int32)), ValueError),
                        (dict(t=T(be, (2, 4))), ValueError), (dict(t=T(be, (3, 4), np.int32)), TypeError),
                        (dict(loss=T(be, (4, 1))), ValueError), (dict(stats=T(be, (1, 4))), ValueError),
@@ -307,7 +308,7 @@ def test_entry_points_check_arguments_before_they_need_a_device():
     good = [P, P, P, P, P, 1.0, 0, 2, 0, 90, 5, 3, 5, s, P, BIG, None]
     ok.append(codes(lib, "nh_distill_fprop", good, [
         {0: None}, {1: None}, {2: None}, {3: None}, {4: None}, {5: 0.0}, {5: -1.0}, {5: float("nan")},
-        {5: float("inf")}, {5: 1e-40}, {6: 3}, {7: 3}, {8: 2}, {9: 0}, {9: 1 << 31}, {10: 1 << 41}, {11: 1025}, {12: 4},
+        {5: float("inf")}, {5: 1e-40}, {5: 1e-20}, {5: 1e20}, {6: 3}, {7: 3}, {8: 2}, {9: 0}, {9: 1 << 31}, {10: 1 << 41}, {11: 1025}, {12: 4},
         {13: None}, {14: None}, {14: P + 8}, {15: lib.nh_distill_workspace_bytes(0, 0, 90, 5) - 1}]))
     #       dz z ids t stats w wall T dtype tdtype axis V N K ldz lddz strides ws bytes stream
     good = [P, P, P, P, P, None, 1.0, 1.0, 0, 2, 0, 90, 5, 3, 5, 5, s, None]

@@ -1018,7 +1018,7 @@ size_t long_row_fprop(int dtype) { return dtype == NH_T_F32 ? 32768 : 65536; }
 // per thread of 1024 spill 61 registers)
 size_t long_row_bprop(int dtype) { return dtype == NH_T_F32 ? 8192 : 16384; }
 // Workgroups that walk over rows.  Forward, threads per CU: 16384 x 5000 bf16 takes 73.4 us with 1024,
-// 73.0 with 2048, 74.6 with 3072 (and 126 with 512, when too few rows are in flight).  Backward, where every
+// 73.0 with 2048 (and 126 with 512, when too few rows are in flight).  Backward, where every
 // workgroup leaves a partial row of both parameter sums: 16384 x 2048 bf16 takes 57 us with 256
 // workgroups, 43 with 512, 46 with 1024, 56 with 2048.
 constexpr size_t FPROP_THREADS = 2048;

@@ -534,8 +534,8 @@ NEON_DEV uint32_t strip_of_block() {
 }
 
 // Running (mean, sum of squared deviations) of two disjoint sets of a column's
-// values joined: with the counts the same for all columns a thread holds, the two
-// factors are computed once.
+// values joined: with the counts the same for all columns a thread holds, the
+// factors are computed once.  A side may be empty: its mean and m2 are 0.
 struct JoinFactors {
     float to_b, cross;      // n_b / n and n_a n_b / n
     NEON_DEV JoinFactors(float na, float nb) {
@@ -543,10 +543,15 @@ struct JoinFactors {
         to_b = n > 0.0f ? nb / n : 0.0f;
         cross = na * to_b;
     }
+    // d * cross before the other d: of an empty side, where cross is 0 and d the other side's mean, nothing
+    // is left whatever the square of d would be.  Where the difference is more than fp32 holds (an infinite
+    // mean among them) the mean is added up from its parts, which leaves infinities what they are.
     NEON_DEV void join(float& mean, float& m2, float mean_b, float m2_b) const {
         const float d = mean_b - mean;
-        mean = __builtin_fmaf(d, to_b, mean);
-        m2 = (m2 + m2_b) + (d * d) * cross;
+        const float parts = __builtin_fmaf(mean, 1.0f - to_b, mean_b * to_b);
+        const float moved = __builtin_fmaf(d, to_b, mean);
+        mean = fabsf(d) <= NH_FLT_MAX ? moved : parts;
+        m2 = (m2 + m2_b) + (d * cross) * d;
     }
 };
 
@@ -601,7 +606,8 @@ template <typename T, int NT, int LC, int RV> struct ColFprop {
             }
         }
     }
-    NEON_DEV void add(uint32_t base, uint32_t end) {
+    // FIRST: there is nothing to join them with
+    template <bool FIRST> NEON_DEV void add(uint32_t base, uint32_t end) {
         int rows = 0;
 #pragma unroll
         for (int i = 0; i < RV; ++i) {
@@ -622,7 +628,12 @@ template <typename T, int NT, int LC, int RV> struct ColFprop {
                 const float d = r[i].get(j) - m;
                 q = __builtin_fmaf(d, i < rows ? d : 0.0f, q);
             }
-            jf.join(mean[j], m2[j], m, q);
+            if constexpr (FIRST) {
+                mean[j] = m;
+                m2[j] = q;
+            } else {
+                jf.join(mean[j], m2[j], m, q);
+            }
         }
         count += (float)rows;
         // (widened again when they are used next: kept as floats they take twice the registers)
@@ -631,17 +642,16 @@ template <typename T, int NT, int LC, int RV> struct ColFprop {
     }
     template <int X> NEON_DEV void fold() {
         if constexpr (X < 64) {
-            const float nb = nh_lane_xor<X>(count);
-            const bool up = (t & X) != 0;
-            // both partners join in the same order, so that they agree to the bit
-            const JoinFactors jf(up ? nb : count, up ? count : nb);
+            // Each side by its share: commutative, so that both partners get the same bits.  The shares are
+            // mostly halves, with which the mean is rounded once; an infinite mean stays one.
+            const float nb = nh_lane_xor<X>(count), n = count + nb;
+            const float mine = n > 0.0f ? count / n : 0.0f, other = n > 0.0f ? nb / n : 0.0f;
+            const float cross = n * (mine * other);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float om = nh_lane_xor<X>(mean[j]), oq = nh_lane_xor<X>(m2[j]);
-                float ma = up ? om : mean[j], qa = up ? oq : m2[j];
-                jf.join(ma, qa, up ? mean[j] : om, up ? m2[j] : oq);
-                mean[j] = ma;
-                m2[j] = qa;
+                const float om = nh_lane_xor<X>(mean[j]), oq = nh_lane_xor<X>(m2[j]), d = om - mean[j];
+                mean[j] = mean[j] * mine + om * other;
+                m2[j] = (m2[j] + oq) + (d * cross) * d;
             }
             count += nb;
             fold<2 * X>();
@@ -714,7 +724,7 @@ template <typename T, int NT, int LC, int RV> __global__ __launch_bounds__(NT, 4
     K k(a, strip_of_block());
     k.load_params(0, a.features);
     k.load(0, a.features);
-    k.add(0, a.features);
+    k.template add<true>(0, a.features);
     k.share(m, k.join(m), true);
     k.put(0, a.features);
 }
@@ -727,9 +737,11 @@ template <typename T> __global__ __launch_bounds__(256) void ln_cols_fprop_sums_
     __shared__ typename K::Shared m;
     K k(a, strip_of_block());
     const uint32_t r0 = blockIdx.y * rows_per, r1 = r0 + rows_per < a.features ? r0 + rows_per : a.features;
-    for (uint32_t base = r0; base < r1; base += K::RL * 8) {
+    k.load(r0, r1);
+    k.template add<true>(r0, r1);
+    for (uint32_t base = r0 + K::RL * 8; base < r1; base += K::RL * 8) {
         k.load(base, r1);
-        k.add(base, r1);
+        k.template add<false>(base, r1);
     }
     const float2 r = k.join(m);
     if (k.t < K::COLS) sums[((size_t)k.strip * chunks + blockIdx.y) * K::COLS + k.t] = r;

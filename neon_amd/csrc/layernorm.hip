@@ -816,10 +816,11 @@ template <typename T, int NT> struct ColBprop {
         float dg = 0.0f, db = 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float d = rd.get(j), e = (rx.get(j) - mu[j]) * d;
+            // (the deviation is normalised first: its product with the error may leave fp32 without that)
+            const float d = rd.get(j), e = (rx.get(j) - mu[j]) * rs[j] * d;
             s1[j] = __builtin_fmaf(d, g, s1[j]);
-            s2[j] = __builtin_fmaf(e, g, s2[j]);           // without the column's factor 1 / std, which share() adds
-            dg = __builtin_fmaf(e, rs[j], dg);
+            s2[j] = __builtin_fmaf(e, g, s2[j]);
+            dg += e;
             db += d;
         }
         // (the sums are in registers here: left to itself the compiler puts these additions off until
@@ -838,9 +839,9 @@ template <typename T, int NT> struct ColBprop {
         o.clear();
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            // s1, s2 as share() leaves them: r mean(u), r^2 mean(u h)
+            // s1, s2 as share() leaves them: r mean(u), r mean(u h)
             const float u = __builtin_fmaf(rd.get(j) * rs[j], g, -s1[j]);
-            o.set(j, __builtin_fmaf(-s2[j], rx.get(j) - mu[j], u));
+            o.set(j, __builtin_fmaf(-s2[j], (rx.get(j) - mu[j]) * rs[j], u));
         }
         store_clipped(o, (T*)a.out + c + (size_t)f * a.ld_out, n);
     }
@@ -910,7 +911,7 @@ template <typename T, int NT> struct ColBprop {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             s1[j] = m.a[0][cl * V + j] * rs[j];
-            s2[j] = m.b[0][cl * V + j] * rs[j] * rs[j] * rs[j];
+            s2[j] = m.b[0][cl * V + j] * rs[j];
         }
     }
 };

@@ -55,3 +55,15 @@ def test_infinite_means_and_variances(hip, f):
                 # an infinite variance: 1 / std is 0
                 assert abs(mean[5]) <= 1e20 and var[5] == np.inf and np.array_equal(y[5], beta[0].astype(np.float32))
 
+
+
+@pytest.mark.parametrize("spread,size", [(1e15, 1e25), (1e-15, 1e-25)])
+@pytest.mark.parametrize("f", [5, 300, 1500, 2500])
+def test_gradients_where_deviation_times_error_leaves_the_range(hip, f, spread, size):
+    """(x - mean) dy alone is outside fp32, the normalised deviation times dy is not"""
+    x, dy, gamma, beta = ln_inputs(9, f, F32, shift=0.0)
+    x, dy = quantise(x * spread, F32), quantise(dy * size, F32)
+    eps = 1e-5 if spread > 1 else float(np.float32(1e-36))
+    for axis in (0, 1):
+        for how in ("plain", "turned"):
+            check_ln(run_ln(hip, x, dy, gamma, beta, axis, how, F32, eps), x, dy, gamma, beta, F32, eps)

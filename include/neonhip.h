@@ -289,8 +289,13 @@ int nh_lut_bprop(void* dW, const void* error_t, const int32_t* ids, int itemsize
  * Workspaces are device scratch on a 16-byte boundary, need not be
  * initialised, and belong to one call at a time: calls that may overlap (other
  * streams, captured graphs) need one each.  No call allocates, synchronises or
- * records a memset.  Arguments are checked before anything is launched.  The
- * kernels run on the device of nh_init.                                        */
+ * records a memset.  Arguments are checked before anything is launched; so is
+ * that every launch's threads can be counted in 32 bits (2^24 workgroups of 256
+ * threads, 2^22 of 1024).  Where a row is a workgroup's that limits the rows:
+ * 2^24 - 1 in distillation and in lookups of 2048 16-bit columns, 2^22 - 1 in layer
+ * normalisation of more than 16384 16-bit features; errors to be turned around
+ * for a table's gradient (axis 0) stay below 64 GiB.  The kernels run on the
+ * device of nh_init.                                                            */
 #define NH_T_F32 0
 #define NH_T_F16 1
 #define NH_T_BF16 2

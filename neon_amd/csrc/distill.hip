@@ -636,8 +636,6 @@ int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* id
     const size_t need = workspace_bytes(dtype, axis, vocab, positions);
     if (!workspace || workspace_bytes_given < need) return lm::refuse(who, "workspace smaller than nh_distill_workspace_bytes");
     if (!lm::aligned16(workspace)) return lm::refuse(who, "workspace off a 16-byte boundary");
-    if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
-    lm::OnDevice here;
     const Chunks c = fprop_chunks(dtype, axis, vocab, positions);
     DistillArgs a = {};
     a.z = z; a.ids = ids; a.t = t; a.loss = loss; a.stats = stats;
@@ -647,22 +645,18 @@ int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* id
     a.stat_k = strides[5]; a.stat_n = strides[6];
     a.part = (nh_pair*)workspace; a.chunk = c.len; a.chunks = c.count;
     a.stream = vocab * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
-    return lm::by_dtype(dtype, [&](auto v) {
-        using T = decltype(v);
-        const hipStream_t s = (hipStream_t)stream;
-        const size_t blocks = (axis == 1 ? positions : lm::ceil_div(positions, strip<T>::COLS)) * c.count;
-        if (blocks > lm::MAX_BLOCKS || positions > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
-        if (axis == 1) hipLaunchKernelGGL((distill_rows_lse_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((distill_cols_lse_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-        if (axis == 0 || c.count > 1) {
+    return lm::run(who, stream, [&](lm::Launches& launch) {
+        lm::by_dtype(dtype, [&](auto v) {
+            using T = decltype(v);
+            if (axis == 1) launch(distill_rows_lse_kernel<T>, positions * c.count, 1, 256, 0, a);
+            else launch(distill_cols_lse_kernel<T>, lm::ceil_div(positions, strip<T>::COLS) * c.count, 1, 256, 0, a);
+            if (axis == 1 && c.count == 1) return;
             // (four positions a wave one after another, or one: 256 positions x 32 entries 4.7 us with one, 11 us
             // with four; 8192 x 256 110 us with one, 53 us with four)
             const uint32_t group = positions >= 4096 ? 16 : 4;
-            hipLaunchKernelGGL((distill_finish_kernel<T>), dim3((unsigned)lm::ceil_div(positions, group)), dim3(256),
-                               (unsigned)(group * entries * 8), s, a, axis == 1 ? ld_z : (size_t)1,
-                               axis == 1 ? (size_t)1 : ld_z, axis == 1, group);
-        }
-        return lm::launched(who);
+            launch(distill_finish_kernel<T>, lm::ceil_div(positions, group), 1, 256, (unsigned)(group * entries * 8), a,
+                   axis == 1 ? ld_z : (size_t)1, axis == 1 ? (size_t)1 : ld_z, axis == 1, group);
+        });
     });
 }
 
@@ -673,8 +667,6 @@ int nh_distill_bprop(void* dz, const void* z, const int32_t* ids, const void* t,
     if (int rc = check(who, dtype, t_dtype, axis, vocab, positions, entries, temperature, ld_z, ld_dz)) return rc;
     if (positions == 0) return 0;
     if (!dz || !stats || !z || !strides || (entries && (!ids || !t))) return lm::refuse(who, "null pointer");
-    if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
-    lm::OnDevice here;
     const Chunks c = bprop_chunks(dtype, axis, vocab, positions);
     DistillArgs a = {};
     a.z = z; a.dz = dz; a.ids = ids; a.t = t; a.stats = const_cast<float*>(stats);
@@ -685,20 +677,13 @@ int nh_distill_bprop(void* dz, const void* z, const int32_t* ids, const void* t,
     a.stat_n = strides[5]; a.weight_n = strides[6];
     a.chunk = c.len; a.chunks = c.count;
     a.stream = 2 * vocab * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
-    return lm::by_dtype(dtype, [&](auto v) {
-        using T = decltype(v);
-        const hipStream_t s = (hipStream_t)stream;
-        const size_t blocks = (axis == 1 ? positions : lm::ceil_div(positions, bstrip<T>::COLS)) * c.count;
-        if (blocks > lm::MAX_BLOCKS || positions > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
-        if (axis == 1) {
-            hipLaunchKernelGGL((distill_rows_bprop_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-        } else {
-            hipLaunchKernelGGL((distill_cols_bprop_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-            if (entries)
-                hipLaunchKernelGGL((distill_patch_kernel<T>), dim3((unsigned)lm::ceil_div(positions, PATCH)), dim3(256),
-                                   (unsigned)patch_lds(entries), s, a);
-        }
-        return lm::launched(who);
+    return lm::run(who, stream, [&](lm::Launches& launch) {
+        lm::by_dtype(dtype, [&](auto v) {
+            using T = decltype(v);
+            if (axis == 1) return launch(distill_rows_bprop_kernel<T>, positions * c.count, 1, 256, 0, a);
+            launch(distill_cols_bprop_kernel<T>, lm::ceil_div(positions, bstrip<T>::COLS) * c.count, 1, 256, 0, a);
+            if (entries) launch(distill_patch_kernel<T>, lm::ceil_div(positions, PATCH), 1, 256, (unsigned)patch_lds(entries), a);
+        });
     });
 }
 

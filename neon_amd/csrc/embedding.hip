@@ -705,27 +705,21 @@ int nh_embed_fprop(void* out, const void* W, const int32_t* ids, float scale, in
     if (int rc = check(who, dtype, axis, positions, embed, vocab, ld_w, ld_out)) return rc;
     if (positions == 0) return 0;
     if (!out || !W || !ids) return lm::refuse(who, "null pointer");
-    if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
-    lm::OnDevice here;
-    const hipStream_t s = (hipStream_t)stream;
-    const uint32_t pad = pad_word(pad_idx);
-    return lm::by_dtype(dtype, [&](auto t) {
-        using T = decltype(t);
-        constexpr size_t V = vec<T>::V;
-        if (axis == 1) {
-            int log = 0;
-            while (log < 8 && ((size_t)V << log) < embed) ++log;
-            const size_t blocks = lm::ceil_div(positions, (size_t)256 >> log);
-            if (blocks > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
-            hipLaunchKernelGGL((lut_rows_fprop_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, (T*)out, (const T*)W, ids,
-                               scale, positions, (uint32_t)embed, (uint32_t)vocab, pad, ld_w, ld_out, log);
-        } else {
-            const size_t blocks = lm::ceil_div(positions, TURN_POS) * lm::ceil_div(embed, 8 * V);
-            if (blocks > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
-            hipLaunchKernelGGL((lut_cols_fprop_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, (T*)out, (const T*)W, ids,
-                               scale, positions, (uint32_t)embed, (uint32_t)vocab, pad, ld_w, ld_out);
-        }
-        return lm::launched(who);
+    const uint32_t pad = pad_word(pad_idx), words = (uint32_t)vocab, cols = (uint32_t)embed;
+    return lm::run(who, stream, [&](lm::Launches& launch) {
+        lm::by_dtype(dtype, [&](auto t) {
+            using T = decltype(t);
+            constexpr size_t V = vec<T>::V;
+            if (axis == 1) {
+                int log = 0;
+                while (log < 8 && ((size_t)V << log) < embed) ++log;
+                launch(lut_rows_fprop_kernel<T>, lm::ceil_div(positions, (size_t)256 >> log), 1, 256, 0, (T*)out, (const T*)W, ids,
+                       scale, positions, cols, words, pad, ld_w, ld_out, log);
+            } else {
+                launch(lut_cols_fprop_kernel<T>, lm::ceil_div(positions, TURN_POS) * lm::ceil_div(embed, 8 * V), 1, 256, 0, (T*)out,
+                       (const T*)W, ids, scale, positions, cols, words, pad, ld_w, ld_out);
+            }
+        });
     });
 }
 
@@ -743,79 +737,73 @@ int nh_embed_update(void* dW, const void* err, const int32_t* ids, float scale, 
     const Layout l = layout(dtype, axis, positions, embed, vocab);
     if (!workspace || workspace_bytes < l.bytes) return lm::refuse(who, "workspace smaller than nh_embed_update_workspace_bytes");
     if (!lm::aligned16(workspace)) return lm::refuse(who, "workspace off a 16-byte boundary");
-    if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
-    lm::OnDevice here;
-    const hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)workspace;
-    return lm::by_dtype(dtype, [&](auto t) {
-        using T = decltype(t);
-        constexpr size_t V = vec<T>::V;
-        SortArgs q = {};
-        q.ids = ids;
-        q.split = (uint2*)(ws + l.split);
-        q.table = (uint32_t*)(ws + l.table);
-        q.scratch = (uint2*)(ws + l.scratch);
-        q.sorted = (uint2*)(ws + l.sorted);
-        q.present = (uint32_t*)(ws + l.present);
-        q.total = (uint32_t*)(ws + l.total);
-        q.count = (uint32_t)positions;
-        q.slices = (uint32_t)lm::ceil_div(positions, SLICE);
-        q.vocab = (uint32_t)vocab;
-        q.pad = pad_word(pad_idx);
-        q.words_per = l.words_per;
-        for (size_t rest = (vocab - 1) >> CLASS_LOG; rest; rest >>= 8) ++q.passes;
-        SumArgs a = {};
-        a.dW = dW;
-        a.err = err;
-        a.ld_err = ld_err;
-        TurnArgs turned = {};
-        size_t turning = 0;
-        if (axis == 0) {
-            turned.from = err;
-            turned.to = ws + l.turned;
-            turned.count = (uint32_t)positions;
-            turned.embed = (uint32_t)embed;
-            turned.tiles_e = (uint32_t)lm::ceil_div(embed, turn<T>::E);
-            turned.ld = ld_err;
-            turning = turned.tiles_e * lm::ceil_div(positions, turn<T>::P);
-            a.err = ws + l.turned;
-            a.ld_err = embed;
-        }
-        if (q.slices + turning > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
-        if (positions)
-            hipLaunchKernelGGL((lut_split_kernel<T>), dim3((unsigned)(q.slices + turning)), dim3(SORT_T), 0, s, q, turned);
-        hipLaunchKernelGGL(lut_class_kernel, dim3(CLASSES), dim3(SORT_T), 0, s, q);
-        a.sorted = q.sorted;
-        a.present = q.present;
-        a.total = q.total;
-        a.joins = (uint4*)(ws + l.joins);
-        a.part = (float*)(ws + l.part);
-        a.scale = scale;
-        a.beta = beta;
-        a.embed = (uint32_t)embed;
-        a.vocab = (uint32_t)vocab;
-        a.words_per = l.words_per;
-        a.ld_dw = ld_dw;
-        a.tiles = (uint32_t)lm::ceil_div(embed, 64 * V);
-        const size_t runs = lm::ceil_div(positions, l.run);
-        a.runs = (uint32_t)runs;
-        const size_t adding = lm::ceil_div(runs * a.tiles, 4), joining = (runs < JOIN_BLOCKS ? runs : JOIN_BLOCKS) * lm::ceil_div(embed, 256);
-        const size_t clearing = beta == 1.0f ? 0 : lm::ceil_div(vocab, 4 * CLEAR_ROWS);
-        const size_t listing = runs > 1 ? lm::ceil_div(runs, 256) : 0;
-        if (listing + adding + clearing > lm::MAX_BLOCKS || joining > lm::MAX_BLOCKS) return lm::refuse(who, "too large for one launch");
-        a.count = (uint32_t)positions;
-        a.list_blocks = (uint32_t)listing;
-        a.sum_blocks = (uint32_t)adding;
-        const auto go = [&](auto run) {
-            constexpr int RUN = decltype(run)::value;
-            if (adding + clearing)
-                hipLaunchKernelGGL((lut_sum_kernel<T, RUN>), dim3((unsigned)(listing + adding + clearing)), dim3(256), 0, s, a);
-            if (runs > 1) hipLaunchKernelGGL((lut_join_kernel<T>), dim3((unsigned)joining), dim3(JOIN_T), 0, s, a);
-        };
-        if (l.run == 32) go(std::integral_constant<int, 32>());
-        else if (l.run == 16) go(std::integral_constant<int, 16>());
-        else go(std::integral_constant<int, 8>());
-        return lm::launched(who);
+    return lm::run(who, stream, [&](lm::Launches& launch) {
+        lm::by_dtype(dtype, [&](auto t) {
+            using T = decltype(t);
+            constexpr size_t V = vec<T>::V;
+            SortArgs q = {};
+            q.ids = ids;
+            q.split = (uint2*)(ws + l.split);
+            q.table = (uint32_t*)(ws + l.table);
+            q.scratch = (uint2*)(ws + l.scratch);
+            q.sorted = (uint2*)(ws + l.sorted);
+            q.present = (uint32_t*)(ws + l.present);
+            q.total = (uint32_t*)(ws + l.total);
+            q.count = (uint32_t)positions;
+            q.slices = (uint32_t)lm::ceil_div(positions, SLICE);
+            q.vocab = (uint32_t)vocab;
+            q.pad = pad_word(pad_idx);
+            q.words_per = l.words_per;
+            for (size_t rest = (vocab - 1) >> CLASS_LOG; rest; rest >>= 8) ++q.passes;
+            SumArgs a = {};
+            a.dW = dW;
+            a.err = err;
+            a.ld_err = ld_err;
+            TurnArgs turned = {};
+            size_t turning = 0;
+            if (axis == 0) {
+                turned.from = err;
+                turned.to = ws + l.turned;
+                turned.count = (uint32_t)positions;
+                turned.embed = (uint32_t)embed;
+                turned.tiles_e = (uint32_t)lm::ceil_div(embed, turn<T>::E);
+                turned.ld = ld_err;
+                turning = turned.tiles_e * lm::ceil_div(positions, turn<T>::P);
+                a.err = ws + l.turned;
+                a.ld_err = embed;
+            }
+            if (positions) launch(lut_split_kernel<T>, q.slices + turning, 1, SORT_T, 0, q, turned);
+            launch(lut_class_kernel, CLASSES, 1, SORT_T, 0, q);
+            a.sorted = q.sorted;
+            a.present = q.present;
+            a.total = q.total;
+            a.joins = (uint4*)(ws + l.joins);
+            a.part = (float*)(ws + l.part);
+            a.scale = scale;
+            a.beta = beta;
+            a.embed = (uint32_t)embed;
+            a.vocab = (uint32_t)vocab;
+            a.words_per = l.words_per;
+            a.ld_dw = ld_dw;
+            a.tiles = (uint32_t)lm::ceil_div(embed, 64 * V);
+            const size_t runs = lm::ceil_div(positions, l.run);
+            a.runs = (uint32_t)runs;
+            const size_t adding = lm::ceil_div(runs * a.tiles, 4), joining = (runs < JOIN_BLOCKS ? runs : JOIN_BLOCKS) * lm::ceil_div(embed, 256);
+            const size_t clearing = beta == 1.0f ? 0 : lm::ceil_div(vocab, 4 * CLEAR_ROWS);
+            const size_t listing = runs > 1 ? lm::ceil_div(runs, 256) : 0;
+            a.count = (uint32_t)positions;
+            a.list_blocks = (uint32_t)listing;
+            a.sum_blocks = (uint32_t)adding;
+            const auto go = [&](auto run) {
+                constexpr int RUN = decltype(run)::value;
+                if (adding + clearing) launch(lut_sum_kernel<T, RUN>, listing + adding + clearing, 1, 256, 0, a);
+                if (runs > 1) launch(lut_join_kernel<T>, joining, 1, JOIN_T, 0, a);
+            };
+            if (l.run == 32) go(std::integral_constant<int, 32>());
+            else if (l.run == 16) go(std::integral_constant<int, 16>());
+            else go(std::integral_constant<int, 8>());
+        });
     });
 }
 

@@ -1110,16 +1110,12 @@ int check(const char* who, int dtype, int axis, size_t features, size_t position
 
 template <typename T> constexpr int code_of() { return sizeof(T) == 4 ? NH_T_F32 : NH_T_F16; }     // (as far as sizes go)
 
-template <typename T> int fprop_rows(const LnArgs& a, hipStream_t s) {
+template <typename T> void fprop_rows(const LnArgs& a, lm::Launches& launch) {
     constexpr size_t V = vec<T>::V;
     const size_t nvec = lm::ceil_div(a.features, V);
-    if (a.positions > lm::MAX_BLOCKS) return lm::refuse("nh_ln_fprop", "too many positions for one launch");
-    if (a.features > long_row_fprop(code_of<T>())) {
-        hipLaunchKernelGGL((ln_rows_fprop_long_kernel<T>), dim3((unsigned)a.positions), dim3(1024), 0, s, a);
-        return lm::launched("nh_ln_fprop");
-    }
-#define LN_WIDE(NV) hipLaunchKernelGGL((ln_rows_fprop_wide_kernel<T, NV>), dim3((unsigned)a.positions), dim3(1024), 0, s, a)
-#define LN_GO(TPR, NV) hipLaunchKernelGGL((ln_rows_fprop_kernel<T, TPR, NV>), dim3(row_blocks(a.positions, TPR, FPROP_THREADS)), dim3(RowShape<TPR>::NT), 0, s, a)
+    if (a.features > long_row_fprop(code_of<T>())) return launch(ln_rows_fprop_long_kernel<T>, a.positions, 1, 1024, 0, a);
+#define LN_WIDE(NV) launch(ln_rows_fprop_wide_kernel<T, NV>, a.positions, 1, 1024, 0, a)
+#define LN_GO(TPR, NV) launch(ln_rows_fprop_kernel<T, TPR, NV>, row_blocks(a.positions, TPR, FPROP_THREADS), 1, RowShape<TPR>::NT, 0, a)
     if (nvec <= 64) LN_GO(64, 1);
     else if (nvec <= 128) LN_GO(64, 2);
     else if (nvec <= 256) LN_GO(256, 1);
@@ -1130,13 +1126,10 @@ template <typename T> int fprop_rows(const LnArgs& a, hipStream_t s) {
     else LN_WIDE(8);
 #undef LN_WIDE
 #undef LN_GO
-    return lm::launched("nh_ln_fprop");
 }
 
-template <typename T> int fprop_cols(const LnArgs& a, hipStream_t s) {
-    const size_t wide = strips_of(COL_FPROP, code_of<T>(), a.positions);
-    if (4 * wide > lm::MAX_BLOCKS) return lm::refuse("nh_ln_fprop", "too many positions for one launch");
-#define LN_GO(NT, LC) hipLaunchKernelGGL((ln_cols_fprop_kernel<T, NT, LC, 8>), dim3((unsigned)lm::ceil_div(a.positions, (LC) * vec<T>::V)), dim3(NT), 0, s, a)
+template <typename T> void fprop_cols(const LnArgs& a, lm::Launches& launch) {
+#define LN_GO(NT, LC) launch(ln_cols_fprop_kernel<T, NT, LC, 8>, lm::ceil_div(a.positions, (LC) * vec<T>::V), 1, NT, 0, a)
     // strips of 128 bytes where four workgroups of them fit a CU (256 x 100352 fp16: 26.1 us, of 64 bytes 30.1),
     // else of 64 (700 x 50000 fp32: 70.1 us, of 128 bytes and 1024 threads 79.7)
     if (a.features <= COL_FPROP.tile) {
@@ -1146,35 +1139,30 @@ template <typename T> int fprop_cols(const LnArgs& a, hipStream_t s) {
     } else if (a.features <= COL_FPROP.resident) {
         LN_GO(1024, 4);
     } else {
+        const size_t strips = strips_of(COL_FPROP, code_of<T>(), a.positions);
         const ColSplit c = split_columns(COL_FPROP, a.features);
-        const dim3 grid((unsigned)wide, c.chunks);
         float2* sums = (float2*)a.part;
-        hipLaunchKernelGGL((ln_cols_fprop_sums_kernel<T>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks, sums);
-        hipLaunchKernelGGL((ln_cols_fprop_finish_kernel<T>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks, (const float2*)sums);
+        launch(ln_cols_fprop_sums_kernel<T>, strips, c.chunks, 256, 0, a, c.rows_per, c.chunks, sums);
+        launch(ln_cols_fprop_finish_kernel<T>, strips, c.chunks, 256, 0, a, c.rows_per, c.chunks, sums);
     }
 #undef LN_GO
-    return lm::launched("nh_ln_fprop");
 }
 
-void add_params(const LnArgs& a, size_t count, hipStream_t s) {
-    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)lm::ceil_div(a.features, 32), 2), dim3(1024), 0, s, a, (uint32_t)count);
+void add_params(const LnArgs& a, size_t count, lm::Launches& launch) {
+    launch(ln_param_kernel, lm::ceil_div(a.features, 32), 2, 1024, 0, a, count);
 }
 
-template <typename T> int bprop_rows(const LnArgs& a, hipStream_t s) {
+template <typename T> void bprop_rows(const LnArgs& a, lm::Launches& launch) {
     constexpr size_t V = vec<T>::V;
-    const size_t nvec = lm::ceil_div(a.features, V);
     const size_t rows = partial_rows(a.features, a.positions, code_of<T>(), false);
     if (a.features > long_row_bprop(code_of<T>())) {
-        if (a.positions > lm::MAX_BLOCKS) return lm::refuse("nh_ln_bprop", "too many positions for one launch");
-        const size_t per = lm::ceil_div(a.positions, rows);
+        const size_t per = lm::ceil_div(a.positions, rows), nvec = lm::ceil_div(a.features, V);
         // (the sums first: dx may take the place of dy)
-        hipLaunchKernelGGL((ln_rows_params_kernel<T>), dim3((unsigned)lm::ceil_div(nvec, 64), (unsigned)rows), dim3(64), 0, s, a, per);
-        hipLaunchKernelGGL((ln_rows_bprop_long_kernel<T>), dim3((unsigned)a.positions), dim3(1024), 0, s, a);
-        add_params(a, rows, s);
-        return lm::launched("nh_ln_bprop");
+        launch(ln_rows_params_kernel<T>, lm::ceil_div(nvec, 64), (unsigned)rows, 64, 0, a, per);
+        launch(ln_rows_bprop_long_kernel<T>, a.positions, 1, 1024, 0, a);
+        return add_params(a, rows, launch);
     }
-    const dim3 grid((unsigned)rows);
-#define LN_GO(TPR, NV) hipLaunchKernelGGL((ln_rows_bprop_kernel<T, TPR, NV>), grid, dim3(RowShape<TPR>::NT), 0, s, a)
+#define LN_GO(TPR, NV) launch(ln_rows_bprop_kernel<T, TPR, NV>, rows, 1, RowShape<TPR>::NT, 0, a)
     if (a.features <= 64 * V) LN_GO(64, 1);
     else if (a.features <= 64 * 8) LN_GO(64, 8 / V < 2 ? 1 : 2);
     else if (a.features <= 64 * 16) LN_GO(64, 16 / V);
@@ -1183,30 +1171,25 @@ template <typename T> int bprop_rows(const LnArgs& a, hipStream_t s) {
     else if (a.features <= 1024 * 8) LN_GO(1024, 8 / V);
     else if constexpr (sizeof(T) == 2) LN_GO(1024, 16 / V);
 #undef LN_GO
-    add_params(a, rows, s);
-    return lm::launched("nh_ln_bprop");
+    add_params(a, rows, launch);
 }
 
-template <typename T> int bprop_cols(LnArgs a, char* ws, hipStream_t s) {
+template <typename T> void bprop_cols(LnArgs a, char* ws, lm::Launches& launch) {
     const size_t strips = strips_of(COL_BPROP, code_of<T>(), a.positions);
-    if (strips > lm::MAX_BLOCKS) return lm::refuse("nh_ln_bprop", "too many positions for one launch");
     float2* sums = (float2*)ws;
     a.part = (float*)(ws + column_sum_bytes(COL_BPROP, a.features, a.positions, code_of<T>()));
-    const dim3 whole((unsigned)strips);
     if (a.features <= 512) {
-        hipLaunchKernelGGL((ln_cols_bprop_kernel<T, 256, 8>), whole, dim3(256), 0, s, a);
+        launch(ln_cols_bprop_kernel<T, 256, 8>, strips, 1, 256, 0, a);
     } else if (a.features <= 1024) {
-        hipLaunchKernelGGL((ln_cols_bprop_kernel<T, 512, 8>), whole, dim3(512), 0, s, a);
+        launch(ln_cols_bprop_kernel<T, 512, 8>, strips, 1, 512, 0, a);
     } else if (a.features <= COL_BPROP.resident) {
-        hipLaunchKernelGGL((ln_cols_bprop_kernel<T, 1024, 8>), whole, dim3(1024), 0, s, a);
+        launch(ln_cols_bprop_kernel<T, 1024, 8>, strips, 1, 1024, 0, a);
     } else {
         const ColSplit c = split_columns(COL_BPROP, a.features);
-        const dim3 grid((unsigned)strips, c.chunks);
-        hipLaunchKernelGGL((ln_cols_bprop_sums_kernel<T>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks, sums);
-        hipLaunchKernelGGL((ln_cols_bprop_finish_kernel<T>), grid, dim3(256), 0, s, a, c.rows_per, c.chunks, (const float2*)sums);
+        launch(ln_cols_bprop_sums_kernel<T>, strips, c.chunks, 256, 0, a, c.rows_per, c.chunks, sums);
+        launch(ln_cols_bprop_finish_kernel<T>, strips, c.chunks, 256, 0, a, c.rows_per, c.chunks, sums);
     }
-    add_params(a, strips, s);
-    return lm::launched("nh_ln_bprop");
+    add_params(a, strips, launch);
 }
 
 }  // namespace
@@ -1228,15 +1211,15 @@ int nh_ln_fprop(void* y, float* mean, float* var, const void* x, const float* ga
     if (need && (!workspace || workspace_bytes_given < need))
         return lm::refuse("nh_ln_fprop", "workspace smaller than nh_ln_workspace_bytes");
     if (!lm::aligned16(workspace)) return lm::refuse("nh_ln_fprop", "workspace off a 16-byte boundary");
-    if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
-    lm::OnDevice here;
     LnArgs a = {};
     a.x = x; a.out = y; a.gamma = gamma; a.beta = beta; a.mean = mean; a.var = var; a.part = (float*)workspace;
     a.eps = eps; a.features = (uint32_t)features; a.positions = positions; a.ld_x = ld_x; a.ld_out = ld_y;
     a.stream = 2 * features * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
-    return lm::by_dtype(dtype, [&](auto t) {
-        using T = decltype(t);
-        return axis == 1 ? fprop_rows<T>(a, (hipStream_t)stream) : fprop_cols<T>(a, (hipStream_t)stream);
+    return lm::run("nh_ln_fprop", stream, [&](lm::Launches& launch) {
+        lm::by_dtype(dtype, [&](auto t) {
+            using T = decltype(t);
+            axis == 1 ? fprop_rows<T>(a, launch) : fprop_cols<T>(a, launch);
+        });
     });
 }
 
@@ -1250,20 +1233,17 @@ int nh_ln_bprop(void* dx, float* dgamma, float* dbeta, const void* dy, const voi
     if (need && (!workspace || workspace_bytes_given < need))
         return lm::refuse("nh_ln_bprop", "workspace smaller than nh_ln_workspace_bytes");
     if (!lm::aligned16(workspace)) return lm::refuse("nh_ln_bprop", "workspace off a 16-byte boundary");
-    if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
-    lm::OnDevice here;
     LnArgs a = {};
     a.x = x; a.dy = dy; a.out = dx; a.gamma = gamma; a.mean = const_cast<float*>(mean); a.var = const_cast<float*>(var);
     a.part = (float*)workspace; a.grads[0] = dgamma; a.grads[1] = dbeta;
     a.eps = eps; a.features = (uint32_t)features; a.positions = positions; a.ld_x = ld_x; a.ld_dy = ld_dy; a.ld_out = ld_dx;
     a.stream = 3 * features * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
-    if (positions == 0) {          // sums over no positions
-        add_params(a, 0, (hipStream_t)stream);
-        return lm::launched("nh_ln_bprop");
-    }
-    return lm::by_dtype(dtype, [&](auto t) {
-        using T = decltype(t);
-        return axis == 1 ? bprop_rows<T>(a, (hipStream_t)stream) : bprop_cols<T>(a, (char*)workspace, (hipStream_t)stream);
+    return lm::run("nh_ln_bprop", stream, [&](lm::Launches& launch) {
+        if (positions == 0) return add_params(a, 0, launch);          // sums over no positions
+        lm::by_dtype(dtype, [&](auto t) {
+            using T = decltype(t);
+            axis == 1 ? bprop_rows<T>(a, launch) : bprop_cols<T>(a, (char*)workspace, launch);
+        });
     });
 }
 

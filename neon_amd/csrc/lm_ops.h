@@ -52,20 +52,54 @@ class OnDevice {
     int back_ = -1;
 };
 
-inline int launched(const char* who) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return nh_internal_fail((int)e, (std::string(who) + ": " + hipGetErrorString(e)).c_str());
-    return 0;
+// What an operator launches.  Its body is gone through twice: to see that the
+// device can count the threads of every launch -- in 32 bits: 2^24 workgroups of
+// 256 threads, 2^22 of 1024 --, and to launch.  So an operator runs as a whole or
+// not at all; should a launch fail all the same, none follows it.
+class Launches {
+  public:
+    Launches(const char* who, hipStream_t stream, bool go) : who_(who), stream_(stream), go_(go) {}
+    // a grid of (blocks, chunks) workgroups
+    template <class... P, class... A>
+    void operator()(void (*kernel)(P...), size_t blocks, unsigned chunks, unsigned threads, unsigned lds, const A&... args) {
+        if (rc_ == 0 && blocks > 0xFFFFFFFFu / threads) rc_ = refuse(who_, "more threads than one launch counts in 32 bits");
+        if (rc_ == 0 && go_) send(kernel, dim3((unsigned)blocks, chunks), dim3(threads), lds, static_cast<P>(args)...);
+    }
+    int status() const { return rc_; }
+
+  private:
+    template <class K, class... P> void send(K kernel, dim3 grid, dim3 block, unsigned lds, P... args) {
+        void* list[] = {&args...};
+        // (the call's own status: what hipGetLastError holds may be another call's)
+        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, list, lds, stream_);
+        if (e == hipSuccess) return;
+        (void)hipGetLastError();
+        rc_ = nh_internal_fail((int)e, (std::string(who_) + ": " + hipGetErrorString(e)).c_str());
+    }
+
+    const char* who_;
+    hipStream_t stream_;
+    bool go_;
+    int rc_ = 0;
+};
+
+template <class F> int run(const char* who, void* stream, F body) {
+    Launches look(who, (hipStream_t)stream, false);
+    body(look);
+    if (look.status()) return look.status();
+    if (!nh_internal_ready()) return nh_internal_fail(NH_ENOTINIT, "nh_init has not been called");
+    OnDevice here;
+    Launches go(who, (hipStream_t)stream, true);
+    body(go);
+    return go.status();
 }
 
 // call f with a value of the storage type `dtype` names
-template <class F> int by_dtype(int dtype, F f) {
-    if (dtype == NH_T_F32) return f(float());
-    if (dtype == NH_T_F16) return f(nh_f16());
-    return f(nh_bf16());
+template <class F> void by_dtype(int dtype, F f) {
+    if (dtype == NH_T_F32) f(float());
+    else if (dtype == NH_T_F16) f(nh_f16());
+    else f(nh_bf16());
 }
-
-constexpr size_t MAX_BLOCKS = 0x7FFFFFFF;
 
 }  // namespace lm
 

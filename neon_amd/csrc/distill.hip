@@ -43,7 +43,6 @@ struct DistillArgs {
     long long loss_n, stat_n, weight_n;
     nh_pair* part;          // forward: (maximum, sum) per position and chunk
     uint32_t chunk, chunks;
-    bool stream;            // the logits are more than the last-level cache holds: read and written past it
 };
 
 NEON_DEV float load_t(const DistillArgs& a, uint32_t k, size_t n) {
@@ -153,9 +152,15 @@ NEON_DEV void finish_position(const DistillArgs& a, size_t n, Lse st, const T* z
     }
 }
 
-template <typename T, int V> NEON_DEV void load_logits(nh_raw<T, V>& r, const T* p, bool stream) {
-    if (stream) r.load_stream(p);
+// PAST: the logits are more than the last-level cache holds, read and written past it.  (A parameter of
+// the kernels: of two branches that differ in that alone the compiler makes one, without it.)
+template <bool PAST, typename T, int V> NEON_DEV void load_logits(nh_raw<T, V>& r, const T* p) {
+    if constexpr (PAST) r.load_stream(p);
     else r.load(p);
+}
+template <bool PAST, typename T, int V> NEON_DEV void store_grads(const nh_out<T, V>& o, T* p) {
+    if constexpr (PAST) o.store_stream(p);
+    else o.store(p);
 }
 
 // ---------------------------------------------------------------------------
@@ -165,7 +170,7 @@ template <typename T, int V> NEON_DEV void load_logits(nh_raw<T, V>& r, const T*
 // TB/s), about half of that time in the exponentials; in chunks of 16 KB 102 us, the
 // fold over the lanes being paid for each.
 // ---------------------------------------------------------------------------
-template <typename T> __global__ __launch_bounds__(256) void distill_rows_lse_kernel(DistillArgs a) {
+template <typename T, bool PAST> __global__ __launch_bounds__(256) void distill_rows_lse_kernel(DistillArgs a) {
     constexpr int V = vec<T>::V, AHEAD = 4;
     __shared__ Lse slots[4];
     const size_t n = blockIdx.x / a.chunks;
@@ -181,7 +186,7 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_lse_ke
     nh_raw<T, V> even[AHEAD], odd[AHEAD];
     const auto load = [&](nh_raw<T, V> (&r)[AHEAD], uint32_t at) {
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) load_logits(r[k], z + at + k * 256 * V, a.stream);
+        for (int k = 0; k < AHEAD; ++k) load_logits<PAST>(r[k], z + at + k * 256 * V);
     };
     const auto add = [&](const nh_raw<T, V> (&r)[AHEAD]) {
         float x[AHEAD * V];
@@ -363,7 +368,7 @@ constexpr int MOST_PLACES = 2 * MOST_ENTRIES;
 
 // One workgroup per position and chunk of the vocabulary: w T q over the chunk,
 // then the few words of the chunk that the teacher names once more with p in.
-template <typename T> __global__ __launch_bounds__(256) void distill_rows_bprop_kernel(DistillArgs a) {
+template <typename T, bool PAST> __global__ __launch_bounds__(256) void distill_rows_bprop_kernel(DistillArgs a) {
     constexpr int V = vec<T>::V, AHEAD = 4;
     __shared__ int ids[MOST_ENTRIES], table[MOST_PLACES];
     __shared__ float ps[MOST_ENTRIES];
@@ -392,7 +397,7 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_bprop_
     nh_raw<T, V> even[AHEAD], odd[AHEAD];
     const auto load = [&](nh_raw<T, V> (&r)[AHEAD], uint32_t at) {
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) load_logits(r[k], z + at + k * 256 * V, a.stream);
+        for (int k = 0; k < AHEAD; ++k) load_logits<PAST>(r[k], z + at + k * 256 * V);
     };
     const auto put = [&](const nh_raw<T, V> (&r)[AHEAD], uint32_t at) {
 #pragma unroll
@@ -401,8 +406,7 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_bprop_
             o.clear();
 #pragma unroll
             for (int j = 0; j < V; ++j) o.set(j, grad(r[k].get(j)));
-            if (a.stream) o.store_stream(dz + at + k * 256 * V);
-            else o.store(dz + at + k * 256 * V);
+            store_grads<PAST>(o, dz + at + k * 256 * V);
         }
     };
     if (batches) load(even, i);
@@ -419,13 +423,13 @@ template <typename T> __global__ __launch_bounds__(256) void distill_rows_bprop_
     for (; i < i1; i += 256 * V) {
         nh_raw<T, V> r;
         const int left = i1 - i < V ? (int)(i1 - i) : V;
-        if (left == V) r.load(z + i);
+        if (left == V) load_logits<PAST>(r, z + i);
         else r.load_partial(z + i, left);
         nh_out<T, V> o;
         o.clear();
 #pragma unroll
         for (int j = 0; j < V; ++j) o.set(j, grad(r.get(j)));
-        if (left == V) o.store(dz + i);
+        if (left == V) store_grads<PAST>(o, dz + i);
         else o.store_partial(dz + i, left);
     }
     if (!some) return;
@@ -484,7 +488,7 @@ template <typename T> __global__ __launch_bounds__(256) void distill_cols_bprop_
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             const T* p = z + (size_t)(i + k * RL < i1 ? i + k * RL : i1 - 1) * a.ld_z;
-            if (n == V) load_logits(r[k], p, a.stream);
+            if (n == V) r[k].load(p);
             else r[k].load_partial(p, n);
         }
     };
@@ -499,7 +503,6 @@ template <typename T> __global__ __launch_bounds__(256) void distill_cols_bprop_
             for (int j = 0; j < V; ++j) o.set(j, some[j] ? w[j] * prob_q(r[k].get(j), a.inv_t, top[j], log_sum[j]) : 0.0f);
             T* p = dz + (size_t)f * a.ld_dz;
             if (n < V) o.store_partial(p, n);
-            else if (a.stream) o.store_stream(p);
             else o.store(p);
         }
     };
@@ -568,7 +571,9 @@ template <typename T> __global__ __launch_bounds__(256) void distill_patch_kerne
 // launch geometry: enough workgroups to fill the device, each with enough of
 // the vocabulary to pay for its share of the teacher's entries
 // ---------------------------------------------------------------------------
-constexpr size_t STREAM_BYTES = (size_t)256 << 20;      // what the last-level cache holds
+// What the last-level cache holds.  Columns are always read and written through the caches: lines that share a
+// cache line with their neighbours' lose by the other way (20828 x 9950 fp16 267 and 303 us).
+constexpr size_t STREAM_BYTES = (size_t)256 << 20;
 
 struct Chunks {
     uint32_t len, count;
@@ -644,11 +649,11 @@ int nh_distill_fprop(float* loss, float* stats, const void* z, const int32_t* id
     a.ids_k = strides[0]; a.ids_n = strides[1]; a.t_k = strides[2]; a.t_n = strides[3]; a.loss_n = strides[4];
     a.stat_k = strides[5]; a.stat_n = strides[6];
     a.part = (nh_pair*)workspace; a.chunk = c.len; a.chunks = c.count;
-    a.stream = vocab * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
+    const bool past = vocab * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
     return lm::run(who, stream, [&](lm::Launches& launch) {
         lm::by_dtype(dtype, [&](auto v) {
             using T = decltype(v);
-            if (axis == 1) launch(distill_rows_lse_kernel<T>, positions * c.count, 1, 256, 0, a);
+            if (axis == 1) launch(past ? distill_rows_lse_kernel<T, true> : distill_rows_lse_kernel<T, false>, positions * c.count, 1, 256, 0, a);
             else launch(distill_cols_lse_kernel<T>, lm::ceil_div(positions, strip<T>::COLS) * c.count, 1, 256, 0, a);
             if (axis == 1 && c.count == 1) return;
             // (four positions a wave one after another, or one: 256 positions x 32 entries 4.7 us with one, 11 us
@@ -676,11 +681,12 @@ int nh_distill_bprop(void* dz, const void* z, const int32_t* ids, const void* t,
     a.ids_k = strides[0]; a.ids_n = strides[1]; a.t_k = strides[2]; a.t_n = strides[3]; a.stat_k = strides[4];
     a.stat_n = strides[5]; a.weight_n = strides[6];
     a.chunk = c.len; a.chunks = c.count;
-    a.stream = 2 * vocab * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
+    const bool past = 2 * vocab * positions * lm::item_bytes(dtype) >= STREAM_BYTES;
     return lm::run(who, stream, [&](lm::Launches& launch) {
         lm::by_dtype(dtype, [&](auto v) {
             using T = decltype(v);
-            if (axis == 1) return launch(distill_rows_bprop_kernel<T>, positions * c.count, 1, 256, 0, a);
+            if (axis == 1)
+                return launch(past ? distill_rows_bprop_kernel<T, true> : distill_rows_bprop_kernel<T, false>, positions * c.count, 1, 256, 0, a);
             launch(distill_cols_bprop_kernel<T>, lm::ceil_div(positions, bstrip<T>::COLS) * c.count, 1, 256, 0, a);
             if (entries) launch(distill_patch_kernel<T>, lm::ceil_div(positions, PATCH), 1, 256, (unsigned)patch_lds(entries), a);
         });

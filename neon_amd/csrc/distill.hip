@@ -166,9 +166,10 @@ template <bool PAST, typename T, int V> NEON_DEV void store_grads(const nh_out<T
 // ---------------------------------------------------------------------------
 // forward: (maximum, sum) of chunks of the vocabulary.  A position whose
 // vocabulary is one chunk is finished by the same workgroup; otherwise one wave
-// per position joins the chunks in order.  4096 x 50001 bf16, 410 MB: 88 us (4.6
-// TB/s), about half of that time in the exponentials; in chunks of 16 KB 102 us, the
-// fold over the lanes being paid for each.
+// per position joins the chunks in order.  4096 x 50001 bf16, 410 MB: 87 us (4.7
+// TB/s), about half of that time in the exponentials; 4096 x 32000 fp32, 524 MB: 87
+// us (6.0 TB/s).  In chunks of 16 KB the former took a seventh more, the fold over
+// the lanes being paid for each.
 // ---------------------------------------------------------------------------
 template <typename T, bool PAST> __global__ __launch_bounds__(256) void distill_rows_lse_kernel(DistillArgs a) {
     constexpr int V = vec<T>::V, AHEAD = 4;
@@ -366,10 +367,13 @@ NEON_DEV bool first_and_sum(const int* ids, const float* ps, uint32_t entries, u
 }
 constexpr int MOST_PLACES = 2 * MOST_ENTRIES;
 
-// One workgroup per position and chunk of the vocabulary: w T q over the chunk,
+// One workgroup per position and chunk of the vocabulary (four 16-byte vectors
+// per thread at most, all asked for before anything else): w T q over the chunk,
 // then the few words of the chunk that the teacher names once more with p in.
+// Bound by HBM: 8192 x 32000 bf16, 1.05 GB: 183 us (5.7 TB/s).
+constexpr size_t ROW_CHUNK_BYTES = 16384;
 template <typename T, bool PAST> __global__ __launch_bounds__(256) void distill_rows_bprop_kernel(DistillArgs a) {
-    constexpr int V = vec<T>::V, AHEAD = 4;
+    constexpr int V = vec<T>::V, VECS = ROW_CHUNK_BYTES / 16 / 256;
     __shared__ int ids[MOST_ENTRIES], table[MOST_PLACES];
     __shared__ float ps[MOST_ENTRIES];
     __shared__ uint32_t twice[MOST_PLACES / 32];
@@ -378,6 +382,13 @@ template <typename T, bool PAST> __global__ __launch_bounds__(256) void distill_
     const uint32_t i1 = i0 + a.chunk < a.vocab ? i0 + a.chunk : a.vocab;
     const T* z = (const T*)a.z + n * a.ld_z;
     T* dz = (T*)a.dz + n * a.ld_dz;
+    // vector k of this thread, of `whole` in the chunk
+    const uint32_t whole = (i1 - i0) / V, rest = (i1 - i0) % V;
+    const auto at = [&](int k) { return k * 256 + threadIdx.x; };
+    nh_raw<T, V> r[VECS];
+#pragma unroll
+    for (int k = 0; k < VECS; ++k)
+        if (at(k) < whole) load_logits<PAST>(r[k], z + i0 + at(k) * V);
     const Stats st = load_stats(a, n);
     const bool some = st.t_top != -NH_INF;
     const float w = weight_of(a, n);
@@ -389,48 +400,18 @@ template <typename T, bool PAST> __global__ __launch_bounds__(256) void distill_
     for (uint32_t k = threadIdx.x; k < places; k += 256) table[k] = -1;
     if (threadIdx.x < places / 32) twice[threadIdx.x] = 0;
     const auto grad = [&](float x) { return some ? w * prob_q(x, a.inv_t, st.top, st.log_sum) : 0.0f; };
-    // batches of AHEAD vectors per thread.  Loads return in the order of issue, stores among them: the
-    // next batch is asked for before this one is stored.
-    constexpr uint32_t BATCH = AHEAD * 256 * V;
-    const uint32_t batches = (i1 - i0) / BATCH;
-    uint32_t i = i0 + threadIdx.x * V;
-    nh_raw<T, V> even[AHEAD], odd[AHEAD];
-    const auto load = [&](nh_raw<T, V> (&r)[AHEAD], uint32_t at) {
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) load_logits<PAST>(r[k], z + at + k * 256 * V);
-    };
-    const auto put = [&](const nh_raw<T, V> (&r)[AHEAD], uint32_t at) {
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            nh_out<T, V> o;
-            o.clear();
-#pragma unroll
-            for (int j = 0; j < V; ++j) o.set(j, grad(r[k].get(j)));
-            store_grads<PAST>(o, dz + at + k * 256 * V);
-        }
-    };
-    if (batches) load(even, i);
-    for (uint32_t b = 0; b < batches; b += 2) {
-        if (b + 1 < batches) load(odd, i + BATCH);
-        put(even, i);
-        if (b + 1 < batches) {
-            if (b + 2 < batches) load(even, i + 2 * BATCH);
-            put(odd, i + BATCH);
-        }
-        i += 2 * BATCH;
-    }
-    i = i0 + batches * BATCH + threadIdx.x * V;
-    for (; i < i1; i += 256 * V) {
-        nh_raw<T, V> r;
-        const int left = i1 - i < V ? (int)(i1 - i) : V;
-        if (left == V) load_logits<PAST>(r, z + i);
-        else r.load_partial(z + i, left);
+    for (int k = 0; k < VECS; ++k) {
+        if (at(k) >= whole) break;
         nh_out<T, V> o;
         o.clear();
 #pragma unroll
-        for (int j = 0; j < V; ++j) o.set(j, grad(r.get(j)));
-        if (left == V) store_grads<PAST>(o, dz + i);
-        else o.store_partial(dz + i, left);
+        for (int j = 0; j < V; ++j) o.set(j, grad(r[k].get(j)));
+        store_grads<PAST>(o, dz + i0 + at(k) * V);
+    }
+    if (threadIdx.x < rest) {        // what is left of a vector, a word each
+        const uint32_t i = i0 + whole * V + threadIdx.x;
+        dz[i] = nh_store_cvt<T>::f(grad((float)z[i]));
     }
     if (!some) return;
     __syncthreads();        // the entries are in LDS, and the chunk is written before its words are written again
@@ -571,14 +552,17 @@ template <typename T> __global__ __launch_bounds__(256) void distill_patch_kerne
 // launch geometry: enough workgroups to fill the device, each with enough of
 // the vocabulary to pay for its share of the teacher's entries
 // ---------------------------------------------------------------------------
-// What the last-level cache holds.  Columns are always read and written through the caches: lines that share a
-// cache line with their neighbours' lose by the other way (20828 x 9950 fp16 267 and 303 us).
+// What the last-level cache holds.  Rows of 32000 bf16 logits, backward: 500 positions (64 MB read and
+// written) 12.1 us through the caches, 14.7 past them; 1000 positions 26.9 and 26.2; 2500 positions 66.0 and
+// 57.4.  Forward: 1500 positions (96 MB) 23.3 and 24.0, 4096 x 50001 90.2 and 86.7.  Columns are always read and written
+// through the caches: lines that share a cache line with their neighbours' lose by the other way (20828 x
+// 9950 fp16 267 and 303 us).
 constexpr size_t STREAM_BYTES = (size_t)256 << 20;
 
 struct Chunks {
     uint32_t len, count;
 };
-constexpr size_t MAX_CHUNKS = (size_t)1 << 31;
+constexpr size_t MAX_CHUNKS = (size_t)1 << 62;        // as many as their least length lets
 Chunks split(size_t vocab, size_t lines, size_t wanted, size_t least) {
     size_t n = lm::ceil_div(wanted, lines ? lines : 1);
     const size_t most = lm::ceil_div(vocab, least);
@@ -594,10 +578,9 @@ Chunks fprop_chunks(int dtype, int axis, size_t vocab, size_t positions) {
     return split(vocab, lm::ceil_div(positions, (size_t)128 / lm::item_bytes(dtype)), 1024, 256);
 }
 Chunks bprop_chunks(int dtype, int axis, size_t vocab, size_t positions) {
-    // rows: 16 KB of logits each, one batch of loads.  Workgroups that come and go sweep the memory in
-    // order (8192 x 32000 bf16: 205 us); with a row each they stay, and 2048 rows in step with one another
-    // take 235 us.
-    if (axis == 1) return split(vocab, positions, MAX_CHUNKS, 16384 / lm::item_bytes(dtype));
+    // rows: what the threads of a workgroup hold at once.  Workgroups that come and go sweep the memory in
+    // order; with a row each they stay, and 2048 rows in step with one another take an eighth longer.
+    if (axis == 1) return split(vocab, positions, MAX_CHUNKS, ROW_CHUNK_BYTES / lm::item_bytes(dtype));
     // columns: 128 words, two batches (20828 x 9950 fp16: 274 us, 256 words 280, 512 words 302)
     return split(vocab, lm::ceil_div(positions, (size_t)256 / lm::item_bytes(dtype)), MAX_CHUNKS, 128);
 }

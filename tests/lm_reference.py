@@ -3,9 +3,11 @@ axis, and how far fp32 arithmetic may be from them.
 
 Bounds.  u = 2^-24 is half a unit of fp32.  A sum of terms t_i in which no term
 passes through more than d additions is off by at most d u sum|t_i| (first
-order); a product or quotient adds u per operation.  ``depth(n)`` bounds d for
-the kernels' sums over n values: a thread adds at most 128 values in a row before
-lanes and waves are joined (6 + 16 additions).  Storage types round once, by at
+order); a product or quotient adds u per operation.  ``depth(n)`` is d for sums over
+n values of which a thread adds at most 128 in a row before lanes and waves are joined (6 + 16
+additions): so it is at the lengths of test_lm_ops.py, and no longer where a thread adds more (dgamma and dbeta:
+a 512th, 256th or 64th of the positions; a vocabulary in one chunk: a 256th of it), which
+test_lm_ops_large.py counts.  Storage types round once, by at
 most ``half(dtype)`` relative, or half the smallest subnormal."""
 import numpy as np
 
@@ -94,7 +96,8 @@ def table_grad(dW, err, ids, scale, beta, pad):
 def table_grad_bound(dW, err, ids, scale, beta, pad):
     vocab = dW.shape[0]
     counts = np.bincount(ids[live(ids, vocab, pad)], minlength=vocab)[:, None]
-    # 32 positions in a row, the partial sums of runs of 32 in eight shares, the shares
+    # 32 positions in a row, the partial sums of runs of 32 in eight shares, the shares (the kernel adds up to 24
+    # partial sums one after another and more in sixteen shares, of runs of 8 to 32: test_lm_ops_large.py)
     d = np.minimum(counts, 32 + (counts // 32 + 2 + 7) // 8 + 8) + 3
     return d * U * np.abs(scale) * table_sums(np.abs(err), ids, vocab, pad) + (2 * U * np.abs(beta * dW) if beta else 0.0)
 

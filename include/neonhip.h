@@ -302,7 +302,7 @@ int nh_lut_bprop(void* dW, const void* error_t, const int32_t* ids, int itemsize
 
 /* y = gamma * (x - mean) / sqrt(var + eps) + beta, mean and var (biased) of each
  * position over its features, written to mean[positions], var[positions];
- * gamma, beta hold one value per feature.  y may be x.                         */
+ * gamma, beta hold one value per feature.  y may be x (with its leading dimension). */
 size_t nh_ln_workspace_bytes(int backward, int dtype, int axis, size_t features, size_t positions);
 int nh_ln_fprop(void* y, float* mean, float* var, const void* x, const float* gamma, const float* beta, float eps,
                 int dtype, int axis, size_t features, size_t positions, size_t ld_x, size_t ld_y,
@@ -310,7 +310,7 @@ int nh_ln_fprop(void* y, float* mean, float* var, const void* x, const float* ga
 /* With h = (x - mean) / sqrt(var + eps), u = gamma * dy:
  *   dx = (u - mean_f(u) - h mean_f(u h)) / sqrt(var + eps),
  *   dgamma = sum over positions of dy h, dbeta = sum over positions of dy
- * (overwritten; added up in a fixed order).  dx may be dy or x.                */
+ * (overwritten; added up in a fixed order).  dx may be dy or x (likewise).      */
 int nh_ln_bprop(void* dx, float* dgamma, float* dbeta, const void* dy, const void* x, const float* mean, const float* var,
                 const float* gamma, float eps, int dtype, int axis, size_t features, size_t positions, size_t ld_x,
                 size_t ld_dy, size_t ld_dx, void* workspace, size_t workspace_bytes, void* stream);

@@ -370,7 +370,7 @@ constexpr int MOST_PLACES = 2 * MOST_ENTRIES;
 // One workgroup per position and chunk of the vocabulary (four 16-byte vectors
 // per thread at most, all asked for before anything else): w T q over the chunk,
 // then the few words of the chunk that the teacher names once more with p in.
-// Bound by HBM: 8192 x 32000 bf16, 1.05 GB: 183 us (5.7 TB/s).
+// Bound by HBM: 8192 x 32000 bf16, 1.05 GB: 178 to 183 us (5.7 to 5.9 TB/s).
 constexpr size_t ROW_CHUNK_BYTES = 16384;
 template <typename T, bool PAST> __global__ __launch_bounds__(256) void distill_rows_bprop_kernel(DistillArgs a) {
     constexpr int V = vec<T>::V, VECS = ROW_CHUNK_BYTES / 16 / 256;
@@ -436,7 +436,8 @@ template <typename T, bool PAST> __global__ __launch_bounds__(256) void distill_
 
 // Columns: w T q everywhere, by strips of 256 bytes of positions and chunks of
 // the vocabulary; distill_patch_kernel writes the teacher's words once more.
-// 20828 x 9950 fp16, 829 MB: 267 us (3.1 TB/s).  Neighbouring workgroups take
+// 20828 x 9950 fp16, 829 MB: 257 us (3.2 TB/s; 1.08 GB moved, lines of 19900 bytes sharing cache lines with
+// their neighbours').  Neighbouring workgroups take
 // neighbouring strips of the same words; with neighbouring chunks of one strip 346
 // us.
 constexpr int BLC = 16;
@@ -573,7 +574,8 @@ Chunks split(size_t vocab, size_t lines, size_t wanted, size_t least) {
 }
 
 Chunks fprop_chunks(int dtype, int axis, size_t vocab, size_t positions) {
-    // (1024 to 8192 workgroups make no difference in columns: 32000 x 8192 bf16 238 to 243 us, with the finish)
+    // (columns with 1024 or 8192 workgroups, with the finish: 32000 x 8192 bf16 and 32 entries 126 and 132 us, 10000 x
+    // 4096 fp32 47.4 and 46.6, 32000 x 256 fp32 15.3 and 15.6)
     if (axis == 1) return split(vocab, positions, 1024, 4096);
     return split(vocab, lm::ceil_div(positions, (size_t)128 / lm::item_bytes(dtype)), 1024, 256);
 }
@@ -581,7 +583,8 @@ Chunks bprop_chunks(int dtype, int axis, size_t vocab, size_t positions) {
     // rows: what the threads of a workgroup hold at once.  Workgroups that come and go sweep the memory in
     // order; with a row each they stay, and 2048 rows in step with one another take an eighth longer.
     if (axis == 1) return split(vocab, positions, MAX_CHUNKS, ROW_CHUNK_BYTES / lm::item_bytes(dtype));
-    // columns: 128 words, two batches (20828 x 9950 fp16: 274 us, 256 words 280, 512 words 302)
+    // columns: 128 words, two batches (us with 128, 256, 512 words: 20828 x 9950 fp16 267, 273, 296; 32000 x 256 fp32
+    // 19.7, 20.1, 23.2; but 32000 x 8192 bf16 297, 250, 249)
     return split(vocab, lm::ceil_div(positions, (size_t)256 / lm::item_bytes(dtype)), MAX_CHUNKS, 128);
 }
 

@@ -36,7 +36,8 @@ NEON_DEV bool in_table(uint32_t w, uint32_t vocab, uint32_t pad) { return w < vo
 
 // ---------------------------------------------------------------------------
 // forward, a position's values side by side: a group of 2^tpr_log threads per
-// position.  Bound by HBM and the caches that hold the frequent rows.
+// position.  Bound by HBM and the caches that hold the frequent rows: 16384 positions
+// x 1024 fp16 of 32000 words 10 us (67 MB read and written, 6.5 TB/s); 65536 x 300 fp32 27 us (157 MB, 5.8 TB/s).
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void lut_rows_fprop_kernel(T* out, const T* W, const int32_t* ids, float scale, size_t count,
@@ -66,7 +67,7 @@ __global__ __launch_bounds__(256) void lut_rows_fprop_kernel(T* out, const T* W,
 }
 
 // forward, positions side by side: tiles of 128 positions and 128 bytes of columns, turned in LDS
-// (16384 positions x 1024 fp16: 11.5 us, 67 MB, 5.8 TB/s)
+// (16384 positions x 1024 fp16: 12 us, 67 MB, 5.6 TB/s)
 constexpr int TURN_POS = 128;
 template <typename T>
 __global__ __launch_bounds__(256) void lut_cols_fprop_kernel(T* out, const T* W, const int32_t* ids, float scale, size_t count,
@@ -651,9 +652,9 @@ struct Layout {
     int run;              // sorted positions per wave of lut_sum_kernel
 };
 
-// Waves of lut_sum_kernel below which it takes shorter runs: eight per CU.  32768 x 1024 bf16 takes 37 us in
-// runs of 32 (2048 waves), 42 in runs of 16, whose partial sums are twice as many; 16384 x 300 fp32 takes
-// 20 us in runs of 32 (1024 waves), 15 in runs of 16, 16 in runs of 8.
+// Waves of lut_sum_kernel below which it takes shorter runs: eight per CU.  Sums + joining in us, in runs of 32,
+// 16 and 8: 32768 x 1024 bf16 (2048 waves of 32) 36 + 6, 39 + 7; 8192 x 4096 bf16 (2048) 72 + 7, 72 + 8; 16384
+// x 300 fp32 (1024) 20 + 5, 15 + 6, 17 + 7; 65536 x 128 fp32 (2048) 34 + 6, 30 + 7.
 constexpr size_t SUM_WAVES = 2048;
 
 Layout layout(int dtype, int axis, size_t count, size_t embed, size_t vocab) {

@@ -100,8 +100,8 @@ template <int TPR> struct RowShape {
 // for before this one is summed up: loads return in the order of issue, stores
 // among them, so a load behind this row's stores would wait for them.  The rows
 // take turns in two sets of registers; moving the next row into this one's place
-// would wait for it.  Bound by HBM: 16384 x 5000 bf16, 328 MB in 66 us (5.0 TB/s; a
-// workgroup per row 84 us, one set of registers 76 us).
+// would wait for it.  Bound by HBM: 16384 x 5000 bf16, 328 MB in 66 to 70 us (4.7 to 5.0
+// TB/s; a workgroup per row 84 us, one set of registers 76 us).
 // ---------------------------------------------------------------------------
 template <typename T, int TPR, int NV> __global__ __launch_bounds__(RowShape<TPR>::NT) void ln_rows_fprop_kernel(LnArgs a) {
     constexpr int V = vec<T>::V, RPB = RowShape<TPR>::RPB;
@@ -290,8 +290,8 @@ template <typename T> __global__ __launch_bounds__(1024) void ln_rows_fprop_long
 // thread, so the sums over positions for dgamma and dbeta stay in registers;
 // each workgroup leaves one partial row of both (gridDim.x of them), which
 // ln_param_kernel adds up in a fixed order.  Bound by HBM: 16384 x 2048 bf16, 201
-// MB in 44 us (4.6 TB/s).  Rows that do not begin on 16 bytes cost about 1.7 times
-// that per byte (7764 x 3356: 2.5 TB/s).
+// MB in 47 us (4.3 TB/s).  Rows that do not begin on 16 bytes cost about 1.7 times
+// that per byte (7764 x 3356: 2.5 TB/s with the sum of the partial rows).
 // ---------------------------------------------------------------------------
 template <typename T, int TPR, int NV> __global__ __launch_bounds__(RowShape<TPR>::NT) void ln_rows_bprop_kernel(LnArgs a) {
     constexpr int V = vec<T>::V, RPB = RowShape<TPR>::RPB;
@@ -414,7 +414,9 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(RowShape<TPR
 }
 
 // rows too long for that: dx in two sweeps per row, the parameter sums by
-// strips of features in a kernel of their own
+// strips of features in a kernel of their own, so that x and dy are read three
+// times, the third out of the caches in part: 4096 x 12000 fp32, 84 + 129 + 5 us for 590 MB that are
+// needed, 1.34 GB moved (6.2 TB/s of those)
 template <typename T> __global__ __launch_bounds__(1024) void ln_rows_bprop_long_kernel(LnArgs a) {
     constexpr int V = vec<T>::V;
     __shared__ float2 slots[16];
@@ -718,6 +720,7 @@ template <typename T, int NT, int LC, int RV> struct ColFprop {
 // The features of a strip in registers: x is read once.  Loads return in the
 // order of issue, stores among them, so gamma and beta are asked for first.
 // 1024 x 25088 fp16, 103 MB: 31 us (3.3 TB/s); in the two-pass form below 33-39 us.
+// Bound by the 64-byte pieces of 50 KB lines.
 template <typename T, int NT, int LC, int RV> __global__ __launch_bounds__(NT, 4) void ln_cols_fprop_kernel(LnArgs a) {
     using K = ColFprop<T, NT, LC, RV>;
     __shared__ typename K::Shared m;
@@ -730,7 +733,8 @@ template <typename T, int NT, int LC, int RV> __global__ __launch_bounds__(NT, 4
 }
 
 // More features than that: statistics of runs of features (blockIdx.y), then the
-// runs' statistics joined in order by every workgroup that finishes one.
+// runs' statistics joined in order by every workgroup that finishes one.  x is read
+// twice: 4096 x 16384 bf16, 38 + 59 us for 269 MB that are needed, 414 moved (4.2 TB/s of those).
 template <typename T> __global__ __launch_bounds__(256) void ln_cols_fprop_sums_kernel(LnArgs a, uint32_t rows_per, uint32_t chunks,
                                                                                       float2* sums) {
     using K = ColFprop<T, 256, 8, 8>;
@@ -985,7 +989,9 @@ template <typename T, int NT, int RV> __global__ __launch_bounds__(NT, 4) void l
 }
 
 // More features than that: column sums of runs of features (blockIdx.y), then
-// the runs' sums joined in order by every workgroup that finishes one.
+// the runs' sums joined in order by every workgroup that finishes one.  x and dy
+// are read twice: 4096 x 16384 bf16, 72 + 87 + 6 us for 403 MB that are needed, 742 moved (4.5
+// TB/s of those).
 template <typename T> __global__ __launch_bounds__(256) void ln_cols_bprop_sums_kernel(LnArgs a, uint32_t rows_per, uint32_t chunks,
                                                                                       float2* sums) {
     using K = ColBprop<T, 256>;
@@ -1030,14 +1036,16 @@ size_t long_row_fprop(int dtype) { return dtype == NH_T_F32 ? 32768 : 65536; }
 // features of a row that the backward kernel holds with its parameter sums (16 fp32 features
 // per thread of 1024 spill 61 registers)
 size_t long_row_bprop(int dtype) { return dtype == NH_T_F32 ? 8192 : 16384; }
-// Workgroups that walk over rows.  Forward, threads per CU: 16384 x 5000 bf16 takes 73.4 us with 1024,
-// 73.0 with 2048 (and 126 with 512, when too few rows are in flight).  Backward, where every
-// workgroup leaves a partial row of both parameter sums: 16384 x 2048 bf16 takes 57 us with 256
-// workgroups, 43 with 512, 46 with 1024, 56 with 2048.
+// Workgroups that walk over rows.  Forward, threads per CU (us with 1024, 2048): 16384 x 5000 bf16 67.8,
+// 68.1; 46000 x 1500 fp32 106, 109; 4096 x 4096 fp32 26.0, 27.5; and the other way 100000 x 100 fp32 19.9,
+// 17.7; 3000 x 600 fp32 6.4, 5.8 (512: 97, 109, 29, 28, 8).
+// Backward, where every workgroup leaves a partial row of both parameter sums (us with 256, 512, 1024
+// workgroups, their sum included): 16384 x 2048 bf16 73.6, 51.4, 52.0; 65536 x 768 bf16 87.2, 62.5, 69.2;
+// 8000 x 4000 fp32 74.6, 78.5, 86.7.
 constexpr size_t FPROP_THREADS = 2048;
 constexpr size_t BPROP_BLOCKS = 512;
-// Rows at least that a workgroup leaves one partial row for (777 x 1537 fp32: 10.5 + 3.7 us with one or two
-// rows each, 8.6 + 2.5 us with three).
+// Rows at least that a workgroup leaves one partial row for (us with 1, 3, 6): 777 x 1537 fp32 14.4, 12.0,
+// 14.8; 512 x 4096 bf16 24.0, 16.3, 17.2; 2048 x 1024 bf16 11.1, 10.7, 14.9.
 constexpr size_t BPROP_ROWS = 3;
 constexpr size_t STREAM_BYTES = (size_t)256 << 20;           // what the last-level cache holds
 constexpr unsigned LONG_ROW_RUNS = 64;        // row runs per feature strip in ln_rows_params_kernel
@@ -1130,8 +1138,9 @@ template <typename T> void fprop_rows(const LnArgs& a, lm::Launches& launch) {
 
 template <typename T> void fprop_cols(const LnArgs& a, lm::Launches& launch) {
 #define LN_GO(NT, LC) launch(ln_cols_fprop_kernel<T, NT, LC, 8>, lm::ceil_div(a.positions, (LC) * vec<T>::V), 1, NT, 0, a)
-    // strips of 128 bytes where four workgroups of them fit a CU (256 x 100352 fp16: 26.1 us, of 64 bytes 30.1),
-    // else of 64 (700 x 50000 fp32: 70.1 us, of 128 bytes and 1024 threads 79.7)
+    // strips of 128 bytes where four workgroups of them fit a CU (256 x 100352 fp16: 26.1 us, of 64 bytes 30.1;
+    // 200 x 25088 bf16 8.8 and 10.9; 256 x 1024 fp32 4.8 and 4.7; 256 x 128 fp32, four workgroups or eight, 4.2
+    // and 4.5), else of 64 (700 x 50000 fp32: 69 us, of 128 bytes and 1024 threads 79.7)
     if (a.features <= COL_FPROP.tile) {
         LN_GO(256, 8);
     } else if (a.features <= 1024) {

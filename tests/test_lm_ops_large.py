@@ -153,3 +153,31 @@ def test_table_gradient_of_frequent_words(hip, name, positions, embed):
         dW = be.empty((vocab, embed), dtype=np_dtype(name))
         be.compound_update_lut(ti, place(be, err, axis, "plain", name), dW, scale=scale, axis=axis)
         ref.within(dW.get(), want, ref.stored(want, name, bound), "table gradient")
+
+
+# words of more than 24 bits take three passes of the sort; more than 4 million positions are more slices than a
+# class's workgroup has threads.  Errors are ones, or the position's parity: sums that fp32 holds exactly
+@pytest.mark.parametrize("vocab,positions,embed,same", [(2 ** 24 + 777, 3000, 3, 0.0), (2 ** 24 + 777, 40000, 2, 0.4),
+                                                        (900, 4300000, 2, 0.1), (70000, 4200001, 1, 0.3)])
+def test_table_gradient_of_large_tables_and_many_positions(hip, vocab, positions, embed, same):
+    be = hip
+    rs = np.random.RandomState(7)
+    ids = rs.randint(0, vocab, positions).astype(np.int32)
+    ids[rs.rand(positions) < same] = vocab - 5                        # a class that does not fit the LDS
+    ids[::1000] = -1
+    ti = be.array(ids.reshape(1, -1), dtype=np.int32)
+    err = np.ones((embed, positions), np.float32)
+    err[-1] = np.arange(positions) % 2
+    ok = ids >= 0
+    want = [np.bincount(ids[ok], weights=err[e][ok], minlength=vocab) for e in range(embed)]
+    for axis in (0, 1):
+        dW = be.empty((vocab, embed))
+        dW[:] = 77.0
+        be.compound_update_lut(ti, be.array(err if axis == 0 else np.ascontiguousarray(err.T)), dW, axis=axis)
+        got = dW.get()
+        for e in range(embed):
+            assert np.array_equal(got[:, e], want[e].astype(np.float32))
+        out = be.empty((embed, positions) if axis == 0 else (positions, embed))
+        be.compound_fprop_lut(ti, dW, out, axis=axis)
+        out = out.get() if axis == 0 else out.get().T
+        assert np.array_equal(out, np.where(ok, got[np.where(ok, ids, 0)].T, 0.0))

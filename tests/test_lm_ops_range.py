@@ -1,10 +1,10 @@
 """Layer normalisation near the ends of the number range: both memory layouts
 give what the formula gives wherever fp32 holds the formula's own steps, and the
-same infinities where it does not."""
+same infinities where it does not.  Distillation at the ends of its temperatures."""
 import numpy as np
 import pytest
 
-from test_lm_ops import BF16, F32, check_ln, ln_inputs, place, quantise, run_ln, vec
+from test_lm_ops import BF16, F16, F32, check_distill, check_ln, distill_inputs, ln_inputs, place, quantise, run_distill, run_ln, vec
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,13 @@ def test_gradients_where_deviation_times_error_leaves_the_range(hip, f, spread, 
     for axis in (0, 1):
         for how in ("plain", "turned"):
             check_ln(run_ln(hip, x, dy, gamma, beta, axis, how, F32, eps), x, dy, gamma, beta, F32, eps)
+
+
+@pytest.mark.parametrize("name", [F32, F16, BF16])
+@pytest.mark.parametrize("tau", [2.0 ** -60, 2.0 ** -20, 2.0 ** 20, 2.0 ** 60])
+def test_distillation_at_the_ends_of_its_temperatures(hip, tau, name):
+    z, ids, t, weight = distill_inputs(9, 700, 11, name, name)
+    if name == F16:
+        weight = weight / max(tau, 1.0)                 # (gradients that the type holds)
+    for axis in (0, 1):
+        check_distill(run_distill(hip, z, ids, t, weight, tau, axis, "plain", name, name), z, ids, t, weight, tau, name)
